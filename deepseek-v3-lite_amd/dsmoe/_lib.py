@@ -7,6 +7,7 @@ unsupported shapes raise ValueError, HIP errors raise RuntimeError.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import warnings
 from pathlib import Path
@@ -41,6 +42,16 @@ class MlaDims(ctypes.Structure):
                 ("R", ctypes.c_int32), ("D_nope", ctypes.c_int32), ("D_rope", ctypes.c_int32),
                 ("D_v", ctypes.c_int32), ("dtype", ctypes.c_int32), ("is_causal", ctypes.c_int32),
                 ("q_start", ctypes.c_int32), ("softmax_scale", ctypes.c_float)]
+
+
+class MlaPagedDims(ctypes.Structure):
+    """dsmoe_mla_paged_dims (include/dsmoe.h)."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("T", "B", "H", "R", "D_nope", "D_rope", "D_v", "pages", "page_size",
+                                               "table_width", "max_q", "max_kv")] +
+                [(n, ctypes.c_int64) for n in ("table_stride", "kv_page_stride", "kv_row_stride", "pe_page_stride",
+                                               "pe_row_stride", "qn_token_stride", "qn_head_stride",
+                                               "qp_token_stride", "qp_head_stride")] +
+                [("softmax_scale", ctypes.c_float)])
 
 
 P = ctypes.c_void_p
@@ -85,6 +96,9 @@ _SIGNATURES = {
     "dsmoe_mla_attn_bwd_workspace_size": ([ctypes.POINTER(MlaDims)], SZ),
     "dsmoe_mla_attn_kv": ([P, P, P, P, ctypes.POINTER(MlaDims), P, SZ, P], I32),
     "dsmoe_mla_attn_bwd": ([P, P, ctypes.POINTER(MlaDims), P, SZ, P, P, P, P, P, P, P, P, SZ, P], I32),
+    "dsmoe_mla_cache_append": ([P, I64, P, I64, I32, P, F32, P, P, P, P, P, ctypes.POINTER(MlaPagedDims), P], I32),
+    "dsmoe_mla_attn_paged_workspace_size": ([ctypes.POINTER(MlaPagedDims)], SZ),
+    "dsmoe_mla_attn_paged": ([P, P, P, P, P, P, P, P, I64, P, I64, ctypes.POINTER(MlaPagedDims), P, P, SZ, P], I32),
 }
 
 _lib = None
@@ -184,6 +198,17 @@ def stream_ptr(device: torch.device):
     """hipStream_t of the device's current stream."""
     index = device.index if device.index is not None else torch.cuda.current_device()
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """A context in which the device is the current one: kernels launch on the current
+    device whatever their stream's."""
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        return _HERE
+    return torch.cuda.device(device)
 
 
 def timing_enable(on: bool) -> None:

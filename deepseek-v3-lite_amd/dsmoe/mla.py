@@ -31,6 +31,8 @@ did not ask for.
 """
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 
 from . import _lib as L
@@ -320,3 +322,151 @@ def mla_attention(q_nope: torch.Tensor, q_pe: torch.Tensor, ctx_kv: torch.Tensor
 
 
 triton_mla_attention = mla_attention
+
+
+# ---------------------------------------------------------------------------- paged latent cache
+# Serving keeps the latent rows of many sequences in pages of one pool.  A call covers the
+# new tokens of a batch of sequences, decoded ones and chunks of prompts alike, packed
+# along the first dimension; three int32 device tensors say which rows are whose:
+#   block_table (B, W)     page of each page_size positions of a sequence
+#   kv_lens     (B,)       positions of a sequence, its new tokens among them
+#   q_offsets   (B + 1,)   rows of sequence b: q_offsets[b] .. q_offsets[b + 1] - 1
+# None is read on the host, so a captured call can be replayed on other lengths and pages.
+def _paged_dims(kv_pages, pe_pages, block_table, kv_lens, q_offsets, T: int, new) -> "L.MlaPagedDims":
+    """The checked description of a paged batch: ValueError on shapes, types or strides the kernels do not take."""
+    dev = kv_pages.device
+    for t in (kv_pages, pe_pages, block_table, kv_lens, q_offsets, *new):
+        if not t.is_cuda:
+            raise RuntimeError("mla_paged: tensors must be on a ROCm GPU (no CPU implementation)")
+        if t.device != dev:
+            raise ValueError("mla_paged: tensors are on different devices")
+    if kv_pages.dtype != torch.bfloat16 or pe_pages.dtype != torch.bfloat16:
+        raise ValueError(f"mla_paged: pages must be bfloat16 (got {kv_pages.dtype}, {pe_pages.dtype})")
+    if kv_pages.dim() != 3 or pe_pages.dim() != 3 or kv_pages.shape[:2] != pe_pages.shape[:2]:
+        raise ValueError("mla_paged: kv_pages must be (pages, page_size, R) and pe_pages (pages, page_size, D_rope), "
+                         f"got {tuple(kv_pages.shape)} and {tuple(pe_pages.shape)}")
+    if kv_pages.stride(2) != 1 or pe_pages.stride(2) != 1:
+        raise ValueError("mla_paged: the rows of the pages must be contiguous")
+    for t, name in ((block_table, "block_table"), (kv_lens, "kv_lens"), (q_offsets, "q_offsets")):
+        if t.dtype != torch.int32:
+            raise ValueError(f"mla_paged: {name} must be int32 (got {t.dtype})")
+    B = kv_lens.size(0) if kv_lens.dim() == 1 else -1
+    if block_table.dim() != 2 or block_table.size(0) != B or q_offsets.dim() != 1 or q_offsets.size(0) != B + 1:
+        raise ValueError("mla_paged: block_table must be (B, W), kv_lens (B,) and q_offsets (B + 1,), got "
+                         f"{tuple(block_table.shape)}, {tuple(kv_lens.shape)} and {tuple(q_offsets.shape)}")
+    if (block_table.stride(1) != 1 and block_table.size(1) > 1) or not kv_lens.is_contiguous() \
+            or not q_offsets.is_contiguous():
+        raise ValueError("mla_paged: kv_lens, q_offsets and the rows of block_table must be contiguous")
+    d = L.MlaPagedDims()
+    d.T, d.B = T, B
+    d.pages, d.page_size, d.R = kv_pages.shape
+    d.D_rope, d.table_width = pe_pages.size(2), block_table.size(1)
+    d.table_stride = block_table.stride(0)
+    d.kv_page_stride, d.kv_row_stride = kv_pages.stride(0), kv_pages.stride(1)
+    d.pe_page_stride, d.pe_row_stride = pe_pages.stride(0), pe_pages.stride(1)
+    return d
+
+
+def _no_grad(what: str, ts) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError(f"{what} has no backward: call it under torch.no_grad(), or detach its inputs")
+
+
+def mla_cache_append(ctx_kv: torch.Tensor, ctx_pe: torch.Tensor, kv_pages: torch.Tensor, pe_pages: torch.Tensor,
+                     block_table: torch.Tensor, kv_lens: torch.Tensor, q_offsets: torch.Tensor, *,
+                     norm_weight: Optional[torch.Tensor] = None, norm_eps: float = 1e-6) -> None:
+    """Writes the latent rows ctx_kv (T, R) and rope rows ctx_pe (T, D_rope) of new tokens into the pages
+    (kv_pages (pages, page_size, R), pe_pages (pages, page_size, D_rope), bf16, any page and row strides), each value
+    rounded to bf16 once; bf16 or fp32 rows.  With norm_weight (R,) the latent row is normed first, in fp32:
+    c rsqrt(mean(c^2) + norm_eps) norm_weight.
+
+    Tokens without a place (rows behind the last sequence, positions before 0 or past the table, pages outside the pool)
+    are skipped.  Pages that the call writes must not be shared: of two tokens with one place either may end there."""
+    _no_grad("mla_cache_append", (ctx_kv, ctx_pe, norm_weight))
+    extra = (ctx_kv, ctx_pe) if norm_weight is None else (ctx_kv, ctx_pe, norm_weight)
+    if ctx_kv.dim() != 2:
+        raise ValueError(f"mla_cache_append: ctx_kv must be (T, R), got {tuple(ctx_kv.shape)}")
+    T, R = ctx_kv.shape
+    d = _paged_dims(kv_pages, pe_pages, block_table, kv_lens, q_offsets, T, extra)
+    if d.R != R or tuple(ctx_pe.shape) != (T, d.D_rope):
+        raise ValueError(f"mla_cache_append: rows {tuple(ctx_kv.shape)}, {tuple(ctx_pe.shape)} for pages of width "
+                         f"{d.R}, {d.D_rope}")
+    if ctx_kv.dtype != ctx_pe.dtype:
+        raise ValueError(f"mla_cache_append: ctx_kv and ctx_pe must share one dtype (got {ctx_kv.dtype}, {ctx_pe.dtype})")
+    if norm_weight is not None:
+        if norm_weight.shape != (R,) or not norm_weight.is_floating_point():
+            raise ValueError(f"mla_cache_append: norm_weight must be ({R},) floating, got {tuple(norm_weight.shape)}")
+        if norm_weight.dtype != torch.float32 or not norm_weight.is_contiguous():
+            norm_weight = norm_weight.float().contiguous()
+    if ctx_kv.stride(1) != 1:
+        ctx_kv = ctx_kv.contiguous()
+    if ctx_pe.stride(1) != 1:
+        ctx_pe = ctx_pe.contiguous()
+    with L.on_device(kv_pages.device):
+        rc = L.load().dsmoe_mla_cache_append(
+            ctx_kv.data_ptr(), ctx_kv.stride(0), ctx_pe.data_ptr(), ctx_pe.stride(0), L.dtype_code(ctx_kv.dtype),
+            L.ptr(norm_weight), norm_eps, kv_pages.data_ptr(), pe_pages.data_ptr(), block_table.data_ptr(),
+            kv_lens.data_ptr(), q_offsets.data_ptr(), d, L.stream_ptr(kv_pages.device))
+    if rc:
+        L.check(rc, "dsmoe_mla_cache_append")
+
+
+def mla_attention_paged(q_nope: torch.Tensor, q_pe: torch.Tensor, kv_pages: torch.Tensor, pe_pages: torch.Tensor,
+                        block_table: torch.Tensor, kv_lens: torch.Tensor, q_offsets: torch.Tensor,
+                        wkv_b_k: torch.Tensor, wkv_b_v: torch.Tensor, softmax_scale: float, *,
+                        max_q: Optional[int] = None, max_kv: Optional[int] = None,
+                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal MLA attention of the new tokens of many sequences over a paged latent cache that holds them already
+    (``mla_cache_append``): q_nope (T, H, D_nope) and q_pe (T, H, D_rope) with any token and head strides, the weights
+    as ``mla_attention`` takes them.  Returns (T, H, D_v) in q_nope's dtype, or writes ``out`` (contiguous bf16).
+
+    max_q and max_kv are the most new tokens and the most positions of a sequence, as the scheduler knows them
+    (default: T, and what the table has room for).  They choose kernels and key ranges; no result rests on them.
+    A token that sees no position gives zeros; rows of ``out`` behind the last sequence stay as they were."""
+    global hip_calls
+    _no_grad("mla_attention_paged", (q_nope, q_pe, kv_pages, pe_pages, wkv_b_k, wkv_b_v, out))
+    out_dtype = q_nope.dtype
+    if q_nope.dim() != 3 or q_pe.dim() != 3 or wkv_b_k.dim() != 3 or wkv_b_v.dim() != 3:
+        raise ValueError("mla_attention_paged: q_nope, q_pe, wkv_b_k and wkv_b_v must have three dimensions")
+    T, H, D_nope = q_nope.shape
+    q_nope, q_pe, wkv_b_k, wkv_b_v = _bf16_inputs((q_nope, q_pe, wkv_b_k, wkv_b_v))
+    d = _paged_dims(kv_pages, pe_pages, block_table, kv_lens, q_offsets, T, (q_nope, q_pe, wkv_b_k, wkv_b_v))
+    R, D_rope, D_v = d.R, d.D_rope, wkv_b_v.size(1)
+    _check_mla_dim_limits(R, D_nope, D_rope, D_v)
+    if tuple(q_pe.shape) != (T, H, D_rope) or tuple(wkv_b_k.shape) != (H, D_nope, R) or wkv_b_v.size(0) != H \
+            or wkv_b_v.size(2) != R:
+        raise ValueError("mla_attention_paged: inconsistent shapes")
+    if q_nope.stride(2) != 1:
+        q_nope = q_nope.contiguous()
+    if q_pe.stride(2) != 1:
+        q_pe = q_pe.contiguous()
+    if not _head_rows(wkv_b_k):
+        wkv_b_k = wkv_b_k.contiguous()
+    if not _head_rows(wkv_b_v):
+        wkv_b_v = wkv_b_v.contiguous()
+    dev = q_nope.device
+    if out is None:
+        res = torch.empty(T, H, D_v, dtype=torch.bfloat16, device=dev)
+    else:
+        if tuple(out.shape) != (T, H, D_v) or out.dtype != torch.bfloat16 or out.device != dev or not out.is_contiguous():
+            raise ValueError(f"mla_attention_paged: out must be a contiguous bfloat16 ({T}, {H}, {D_v}) on {dev}")
+        res = out
+    d.H, d.D_nope, d.D_v = H, D_nope, D_v
+    d.max_q = T if max_q is None else min(int(max_q), T)
+    room = d.table_width * d.page_size
+    d.max_kv = min(room if max_kv is None else int(max_kv), room, 0x7fffffff)
+    d.qn_token_stride, d.qn_head_stride = q_nope.stride(0), q_nope.stride(1)
+    d.qp_token_stride, d.qp_head_stride = q_pe.stride(0), q_pe.stride(1)
+    d.softmax_scale = softmax_scale
+    lib = L.load()
+    nbytes = lib.dsmoe_mla_attn_paged_workspace_size(d)
+    with L.on_device(dev):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        rc = lib.dsmoe_mla_attn_paged(
+            q_nope.data_ptr(), q_pe.data_ptr(), kv_pages.data_ptr(), pe_pages.data_ptr(), block_table.data_ptr(),
+            kv_lens.data_ptr(), q_offsets.data_ptr(), wkv_b_k.data_ptr(), wkv_b_k.stride(0), wkv_b_v.data_ptr(),
+            wkv_b_v.stride(0), d, res.data_ptr(), ws.data_ptr(), nbytes, L.stream_ptr(dev))
+    if rc:
+        L.check(rc, "dsmoe_mla_attn_paged")
+    hip_calls += 1
+    return res if out is not None or out_dtype == torch.bfloat16 else res.to(out_dtype)

@@ -366,6 +366,60 @@ int dsmoe_mla_attn_bwd(const void* q_nope, const void* q_pe, const dsmoe_mla_dim
                        float* dq_pe, void* dkv, float* dk_pe, void* workspace, size_t workspace_bytes,
                        void* stream);
 
+/* ---------------------------------------------------------------------------
+ * A paged latent cache, its writes and the attention of new tokens over it.  No
+ * counterpart in the reference, which keeps one contiguous cache per batch row and
+ * assigns slices of it (models/mla.py:95-125); the attention is that of
+ * dsmoe_mla_attn_fwd with the causal mask.
+ *
+ * B sequences have new tokens, packed as rows of T: sequence b's are the rows
+ * q_offsets[b] .. q_offsets[b + 1] - 1 (q_offsets (B + 1) int32, not decreasing), and
+ * kv_lens[b] (B int32) positions belong to it with them, so its new token i stands at
+ * position kv_lens[b] - (its new tokens) + i.  Position p lies on page
+ * block_table[b][p / page_size] (int32, rows table_stride entries apart, table_width
+ * entries each) at row p % page_size of it.  All of these are device arrays; no call
+ * reads them on the host.  What they may hold without harm: a sequence without new
+ * tokens or without positions, more positions than the table has room for (those past it
+ * hold no key and take no row), fewer positions than new tokens (a token before position
+ * 0 is not written and sees nothing), a page outside [0, pages) (likewise).  Rows of T
+ * behind the last sequence are neither read as queries nor written.  Strides count
+ * elements; rows are contiguous.
+ */
+typedef struct dsmoe_mla_paged_dims {
+  int32_t T, B;
+  int32_t H, R, D_nope, D_rope, D_v;   /* H, D_nope, D_v: the attention's alone */
+  int32_t pages, page_size, table_width;
+  int32_t max_q;    /* most new tokens of a sequence, and */
+  int32_t max_kv;   /* most positions: they choose kernels and ranges (speed), no result rests on them */
+  int64_t table_stride;
+  int64_t kv_page_stride, kv_row_stride;   /* kv_pages (pages, page_size, R) bf16 */
+  int64_t pe_page_stride, pe_row_stride;   /* pe_pages (pages, page_size, D_rope) bf16 */
+  int64_t qn_token_stride, qn_head_stride; /* q_nope (T, H, D_nope) bf16 */
+  int64_t qp_token_stride, qp_head_stride; /* q_pe (T, H, D_rope) bf16 */
+  float softmax_scale;
+} dsmoe_mla_paged_dims;
+
+/* Writes the new rows ctx_kv (T, R) and ctx_pe (T, D_rope), of type dtype and rows
+ * *_stride elements apart, to their positions, each value rounded to bf16 once.  With
+ * norm_weight (R fp32, may be NULL) the latent row is normed first:
+ * c rsqrt(mean(c^2) + norm_eps) norm_weight, in fp32.  Where two tokens have the same
+ * place (a page twice in the tables) either row may end there, whole or mixed. */
+int dsmoe_mla_cache_append(const void* ctx_kv, int64_t ctx_kv_stride, const void* ctx_pe, int64_t ctx_pe_stride,
+                           int dtype, const float* norm_weight, float norm_eps, void* kv_pages, void* pe_pages,
+                           const int32_t* block_table, const int32_t* kv_lens, const int32_t* q_offsets,
+                           const dsmoe_mla_paged_dims* dims, void* stream);
+
+/* out (T, H, D_v) bf16: every new token's attention over the positions up to its own
+ * (zeros where there is none), dims and weights as dsmoe_mla_attn_fwd_heads (R, D_* <= 256,
+ * D_nope + D_rope <= 256); T H < 2^24.  A NaN or an infinity in a cached row reaches the tokens that
+ * see it and no other. */
+size_t dsmoe_mla_attn_paged_workspace_size(const dsmoe_mla_paged_dims* dims);
+int dsmoe_mla_attn_paged(const void* q_nope, const void* q_pe, const void* kv_pages, const void* pe_pages,
+                         const int32_t* block_table, const int32_t* kv_lens, const int32_t* q_offsets,
+                         const void* wkv_b_k, int64_t wk_head_stride, const void* wkv_b_v, int64_t wv_head_stride,
+                         const dsmoe_mla_paged_dims* dims, void* out, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif
