@@ -44,6 +44,12 @@ class MlaDims(ctypes.Structure):
                 ("q_start", ctypes.c_int32), ("softmax_scale", ctypes.c_float)]
 
 
+class RouteDims(ctypes.Structure):
+    """dsmoe_route_dims (include/dsmoe.h)."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("T", "E", "k", "score", "n_groups", "topk_groups", "group_top2",
+                                               "normalise")] + [("route_scale", ctypes.c_float)])
+
+
 class MlaPagedDims(ctypes.Structure):
     """dsmoe_mla_paged_dims (include/dsmoe.h)."""
     _fields_ = ([(n, ctypes.c_int32) for n in ("T", "B", "H", "R", "D_nope", "D_rope", "D_v", "pages", "page_size",
@@ -96,6 +102,8 @@ _SIGNATURES = {
     "dsmoe_mla_attn_bwd_workspace_size": ([ctypes.POINTER(MlaDims)], SZ),
     "dsmoe_mla_attn_kv": ([P, P, P, P, ctypes.POINTER(MlaDims), P, SZ, P], I32),
     "dsmoe_mla_attn_bwd": ([P, P, ctypes.POINTER(MlaDims), P, SZ, P, P, P, P, P, P, P, P, SZ, P], I32),
+    "dsmoe_route_experts": ([P, P, ctypes.POINTER(RouteDims), P, P, P, P], I32),
+    "dsmoe_route_experts_bwd": ([P, P, P, ctypes.POINTER(RouteDims), P, P], I32),
     "dsmoe_mla_cache_append": ([P, I64, P, I64, I32, P, F32, P, P, P, P, P, ctypes.POINTER(MlaPagedDims), P], I32),
     "dsmoe_mla_attn_paged_workspace_size": ([ctypes.POINTER(MlaPagedDims)], SZ),
     "dsmoe_mla_attn_paged": ([P, P, P, P, P, P, P, P, I64, P, I64, ctypes.POINTER(MlaPagedDims), P, P, SZ, P], I32),

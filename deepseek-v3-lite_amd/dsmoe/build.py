@@ -36,7 +36,7 @@ CFLAGS = [
 EXTRA_FLAGS = {"mla.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "mla_few.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                "mla_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 SOURCES = ["api.hip", "gate.hip", "permute.hip", "gemm.hip", "gemm_f32.hip", "gemm_qp.hip", "gemm_sk.hip", "gemm_x.hip", "gemm_xm.hip", "gemm_xq.hip", "bwd.hip", "combine.hip", "mla.hip", "mla_few.hip",
-           "mla_cache.hip", "mla_paged.hip"]
+           "mla_cache.hip", "mla_paged.hip", "route_experts.hip"]
 PROBE_SOURCES = ["probe.hip"]
 
 

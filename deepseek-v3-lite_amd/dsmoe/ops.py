@@ -4,6 +4,7 @@
 * ``grouped_moe_dispatch`` the operator seam of models/moe_triton.py:504-525
 * ``gate_forward``, ``route_from_logits``, ``permute``, ``combine``:
   the individual stages, exposed for tests and for callers that compose them.
+* ``route_experts``        routing from logits with softmax scores, groups of experts and its gradient
 
 Every function requires ROCm device tensors and the built HIP library; there
 is no CPU path.
@@ -83,6 +84,91 @@ def route_from_logits(logits: torch.Tensor, gate_bias: torch.Tensor, k: int, rou
                                           L.ptr(out["counts"]), L.stream_ptr(dev))
     L.check(rc, "dsmoe_route_from_logits")
     return out
+
+
+_SCORES = {"sigmoid": 0, "softmax": 1}
+_GROUP_SCORES = {"max": 0, "top2": 1}
+
+
+def _route_fwd(logits, bias, d):
+    T, E, k, dev = d.T, d.E, d.k, logits.device
+    weights = torch.empty(T, k, dtype=torch.float32, device=dev)
+    idx = torch.empty(T, k, dtype=torch.int32, device=dev)
+    counts = torch.empty(E, dtype=torch.int32, device=dev)
+    with L.on_device(dev):
+        rc = L.load().dsmoe_route_experts(logits.data_ptr(), L.ptr(bias), d, weights.data_ptr(), idx.data_ptr(),
+                                          counts.data_ptr(), L.stream_ptr(dev))
+    if rc:
+        L.check(rc, "dsmoe_route_experts")
+    return weights, idx, counts
+
+
+class _RouteFn(torch.autograd.Function):
+    """dsmoe_route_experts under autograd: the weights carry the gradient of the logits."""
+
+    @staticmethod
+    def forward(ctx, logits, bias, d):
+        ctx.dtype, ctx.d = logits.dtype, d
+        logits = _c(logits.float())
+        weights, idx, counts = _route_fwd(logits, bias, d)
+        ctx.save_for_backward(logits, idx)
+        ctx.mark_non_differentiable(idx, counts)
+        ctx.set_materialize_grads(False)
+        return weights, idx, counts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dweights, _didx, _dcounts):
+        if dweights is None:
+            return None, None, None
+        logits, idx = L.restored(ctx.saved_tensors)
+        dev = logits.device
+        dweights = _c(dweights.float())
+        dlogits = torch.empty_like(logits)
+        with L.on_device(dev):
+            rc = L.load().dsmoe_route_experts_bwd(logits.data_ptr(), idx.data_ptr(), dweights.data_ptr(), ctx.d,
+                                                  dlogits.data_ptr(), L.stream_ptr(dev))
+        if rc:
+            L.check(rc, "dsmoe_route_experts_bwd")
+        return dlogits if ctx.dtype == torch.float32 else dlogits.to(ctx.dtype), None, None
+
+
+def route_experts(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None, *, score: str = "sigmoid",
+                  n_groups: int = 1, topk_groups: Optional[int] = None, group_score: str = "top2",
+                  normalise: bool = True, route_scale: float = 1.0):
+    """Routing of T tokens to k of E experts from logits (T, E): (weights (T, k) fp32, idx (T, k) int32, counts (E,) int32).
+
+    score       "sigmoid" or "softmax" of the logits, in 64 bits, rounded once
+    bias        (E,) fp32, added to the scores for the choice alone (no gradient)
+    n_groups    groups of consecutive experts, of which the topk_groups best (default: all) stay; a group's
+                group_score is the sum of its two largest biased scores ("top2") or its largest ("max")
+    normalise   weights divided by their sum (at least 1e-10)
+    Equal scores go to the lower group or expert, NaN comes last.  The weights are differentiable in the logits (closed
+    form, dense for softmax scores).  With the defaults weights and idx are route_from_logits' bit for bit.  E <= 512, k <= 16,
+    n_groups <= 64; ValueError otherwise."""
+    if bias is None:
+        dev = _require_gpu(logits)
+    else:
+        dev = _require_gpu(logits, bias)
+        if bias.device != dev:
+            raise ValueError("route_experts: logits and bias are on different devices")
+    if logits.dim() != 2 or not logits.is_floating_point():
+        raise ValueError(f"route_experts: logits must be floating (T, E), got {logits.dtype} {tuple(logits.shape)}")
+    T, E = logits.shape
+    if score not in _SCORES or group_score not in _GROUP_SCORES:
+        raise ValueError(f"route_experts: score must be one of {tuple(_SCORES)} and group_score of {tuple(_GROUP_SCORES)}, "
+                         f"got {score!r} and {group_score!r}")
+    if bias is not None:
+        if tuple(bias.shape) != (E,):
+            raise ValueError(f"route_experts: bias must be ({E},), got {tuple(bias.shape)}")
+        bias = bias.detach()
+        if bias.dtype != torch.float32 or not bias.is_contiguous():
+            bias = bias.float().contiguous()
+    d = L.RouteDims(T, E, int(k), _SCORES[score], int(n_groups), int(n_groups if topk_groups is None else topk_groups),
+                    _GROUP_SCORES[group_score], 1 if normalise else 0, float(route_scale))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _RouteFn.apply(logits, bias, d)
+    return _route_fwd(_c(logits.detach().float()), bias, d)
 
 
 def check_routing(idx: torch.Tensor, E: int) -> None:

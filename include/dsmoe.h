@@ -420,6 +420,38 @@ int dsmoe_mla_attn_paged(const void* q_nope, const void* q_pe, const void* kv_pa
                          const dsmoe_mla_paged_dims* dims, void* out, void* workspace, size_t workspace_bytes,
                          void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Routing to experts from fp32 logits (T, E), and its gradient: the part of
+ * models/moe.py:32-36 after F.linear with more kinds of scores and choices than
+ * dsmoe_route_from_logits, whose results it gives bit for bit for sigmoid scores, one
+ * group and normalised weights.
+ *   s = sigmoid(l) or softmax(l), evaluated in double and rounded once to fp32;
+ *   c = s + bias (bias (E) fp32, may be NULL);
+ *   n_groups groups of E / n_groups consecutive experts: a group's score is the fp32 sum
+ *     of its two largest c (group_top2; of a group of one expert its c) or its largest;
+ *     the topk_groups best stay, equal scores by the lower group;
+ *   k of their experts in descending c; equal values by the lower id, NaN last;
+ *   weights (T, k) fp32 = s_j / max(sum_j s_j, 1e-10) route_scale (normalise), or
+ *     s_j route_scale;  idx (T, k) int32;  counts (E) int32, may be NULL.
+ * The backward takes the forward's logits and idx and dweights (T, k) fp32, and writes
+ * dlogits (T, E) fp32 (the choice, the bias and counts carry no gradient).
+ * E <= 512, k <= 16, n_groups <= 64. */
+#define DSMOE_SCORE_SIGMOID 0
+#define DSMOE_SCORE_SOFTMAX 1
+#define DSMOE_ROUTE_MAX_EXPERTS 512
+typedef struct dsmoe_route_dims {
+  int32_t T, E, k;
+  int32_t score;
+  int32_t n_groups, topk_groups;
+  int32_t group_top2;
+  int32_t normalise;
+  float route_scale;
+} dsmoe_route_dims;
+int dsmoe_route_experts(const float* logits, const float* bias, const dsmoe_route_dims* dims, float* weights,
+                        int32_t* idx, int32_t* counts, void* stream);
+int dsmoe_route_experts_bwd(const float* logits, const int32_t* idx, const float* dweights,
+                            const dsmoe_route_dims* dims, float* dlogits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
