@@ -280,38 +280,6 @@ constexpr int MLB_KW = 128;   // keys per workgroup of the dK, dV kernel
 constexpr int MLB_QI = 64;    // queries per staged tile of the dK, dV kernel (two halves of 32)
 constexpr int MLB_KT = 64;    // keys per staged tile of the dQ kernel
 
-// ---------------------------------------------------------------- work items
-// The attention kernels' work items are (batch-head pair hb, rank) with rank
-// r the r-th longest of a pair's items under the causal mask (the forward
-// and dQ kernels: query blocks from the last; the dK, dV kernel: key blocks
-// from the first).  Block i runs on XCD i % 8 (local index j = i / 8).  With
-// at least MLA_SPREAD pairs, XCD x owns the pairs x, x + 8, ... (their K, V
-// or query-side rows share its L2) and walks them rank-major, so the
-// dispatcher, which starts blocks in order as slots free up, runs every
-// pair's longest item first and the short ones fill the tail.  Fewer pairs:
-// the XCDs take contiguous eighths of the pair-major list (every XCD busy).
-// Grid: 8 * ceil(BH / 8) * nrank blocks; false for a block past the items.
-constexpr int MLA_SPREAD = 32;
-
-__device__ __forceinline__ bool mla_item(int blk, int BH, int nrank, int& hb, int& rank) {
-  const int x = blk & 7, j = blk >> 3;
-  if (BH >= MLA_SPREAD) {
-    const int nh = (BH - x + 7) >> 3;   // pairs on this XCD
-    if (j >= nh * nrank) return false;
-    rank = j / nh;
-    hb = x + 8 * (j - rank * nh);
-    return true;
-  }
-  const int total = BH * nrank, per = (total + 7) / 8;
-  const int item = x * per + j;
-  if (j >= per || item >= total) return false;
-  hb = item / nrank;
-  rank = item - hb * nrank;
-  return true;
-}
-
-__host__ __device__ inline int64_t mla_grid(int BH, int nrank) { return 8 * (int64_t)((BH + 7) / 8) * nrank; }
-
 // ---------------------------------------------------------------- attention
 // LDS per buffer: K tile 64 x KRB bytes in the mlb_off layout, then V tile
 // 64 x DVp * 2 bytes with 8-byte unit u of key row k stored at
@@ -319,11 +287,6 @@ __host__ __device__ inline int64_t mla_grid(int BH, int nrank) { return 8 * (int
 // key rows and eight units each, which this spreads over distinct banks.  The
 // swizzle moves whole 16-byte chunks (it is a multiple of 8 units), so a tile
 // arrives by direct 16-byte loads.
-template <int NV>
-__device__ __forceinline__ int mla_vswz(int k) {
-  return NV == 1 ? 0 : NV == 2 ? 8 * ((k >> 1) & 1) : 8 * (k & 3);
-}
-
 template <int NSTEP, int NV>
 struct MlaCfg {
   static constexpr int DQKp = NSTEP * 16;

@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void mla_cache_append_kernel(const CacheArgs a
       cache_ld8<T>(a.ctx_kv, t * a.ckv_rs + c8, v);
     if (a.norm_w && !pe_side) cache_ld8<float>(a.norm_w, c8, w);
   }
-  const PagedSeq s = paged_seq(a.p, paged_find(a.p, t, 1, 1, 0));
+  const PagedSeq s = paged_seq(a.p, paged_find(a.p, a.p.offsets, t, 1, 1, 0));
   const int pos = s.first + t - s.t0;
   // rows behind the last sequence, and positions without a place, are left alone
   if (s.b < 0 || t - s.t0 >= s.n || pos < 0 || pos >= s.kv) return;
@@ -117,7 +117,7 @@ int paged_validate(const dsmoe_mla_paged_dims* d) {
 PagedBatch paged_batch(const dsmoe_mla_paged_dims* d, const int32_t* table, const int32_t* kv_lens,
                        const int32_t* offsets) {
   PagedBatch p;
-  p.table = table; p.kv_lens = kv_lens; p.offsets = offsets;
+  p.table = table; p.kv_lens = kv_lens; p.offsets = p.rows = offsets;
   p.table_stride = d->table_stride;
   p.kv_ps = d->kv_page_stride; p.kv_rs = d->kv_row_stride;
   p.pe_ps = d->pe_page_stride; p.pe_rs = d->pe_row_stride;

@@ -21,6 +21,7 @@
 // reaches those and no other.
 #include <algorithm>
 #include <cfloat>
+#include <climits>
 #include <cstring>
 
 #include "mla_paged.h"
@@ -29,29 +30,6 @@
 namespace dsmoe {
 
 constexpr int PG_MAX_SPLITS = 128;
-
-struct PagedAttn {
-  PagedBatch p;
-  const bf16_t* q_nope;   // row of token t, head h at t qn_ts + h qn_hs
-  const bf16_t* q_pe;
-  int64_t qn_ts, qn_hs, qp_ts, qp_hs;
-  const bf16_t* kv_pages;
-  const bf16_t* pe_pages;
-  const bf16_t* w_k;      // head h's (Dn, R) rows at h wk_hs
-  const bf16_t* w_v;      // head h's (Dv, R) rows at h wv_hs
-  int64_t wk_hs, wv_hs;
-  bf16_t* out;            // (T, H, Dv)
-  bf16_t* qabs;           // (T H, 2 Rq + Drp): [hi | lo | pe], zeros in the padding
-  float* po;              // (nsplit, T H, Rq) partial sums of p c
-  float2* ml;             // (nsplit, T H) {max of the scores, sum of p}
-  int H, R, Dn, Dr, Dv;
-  int Rq, Drp;            // R and Dr in whole MFMA steps
-  int tiles;              // bound of the tile numbers
-  int nsplit, cpw;        // key ranges, and 32-key chunks of each but the last
-  int neg;                // softmax_scale < 0: q is negated, c = |scale| log2(e)
-  int wvec;               // 16-byte loads of weight rows
-  float c;
-};
 
 // 8 bf16 at p (16 bytes), or those of p[0 .. n) one by one and zeros.
 __device__ __forceinline__ bf16x8_t pg_ld8(const bf16_t* p, int n, bool vec) {
@@ -69,7 +47,7 @@ __device__ __forceinline__ bf16x8_t pg_ld8(const bf16_t* p, int n, bool vec) {
 
 // The first position that no row of tile mt sees (0: nothing to see).
 __device__ __forceinline__ int pg_kend(const PagedSeq& s, int H, int mt) {
-  return max(0, min(s.kv, s.first + (min(s.n * H, 32 * mt + 32) - 1) / H + 1));
+  return max(0, min(s.kv, s.first + (min(s.m * H, 32 * mt + 32) - 1) / H + 1));
 }
 
 // Key ranges that hold keys, of a tile that sees kend of them.
@@ -77,14 +55,17 @@ __device__ __forceinline__ int pg_ranges(const PagedAttn& a, int kend) {
   return min(a.nsplit, (kend + 32 * a.cpw - 1) / (32 * a.cpw));
 }
 
-// Grid (T, H).  Thread (g, c): columns 8 c .. 8 c + 7 over the D_nope rows g,
-// g + groups, ..., the groups added through LDS.
-__global__ __launch_bounds__(256) void paged_absorb_kernel(const PagedAttn a) {
+__device__ __forceinline__ void paged_absorb_row(const PagedAttn& a, int rt, int h) {
   extern __shared__ __attribute__((aligned(16))) float pg_sm[];
-  const int tid = threadIdx.x, t = blockIdx.x, h = blockIdx.y;
+  const int tid = threadIdx.x;
+  int t = rt;
+  if (a.p.rows != a.p.offsets) {
+    const PagedSeq s = paged_seq(a.p, paged_find(a.p, a.p.rows, rt, 1, 1, 0));
+    t = s.t0 + rt - s.r0;
+  }
   const bf16_t* qn = a.q_nope + t * a.qn_ts + h * a.qn_hs;
   const bf16_t* qp = a.q_pe + t * a.qp_ts + h * a.qp_hs;
-  bf16_t* dst = a.qabs + ((int64_t)t * a.H + h) * (2 * a.Rq + a.Drp);
+  bf16_t* dst = a.qabs + ((int64_t)rt * a.H + h) * (2 * a.Rq + a.Drp);
   const int cols = a.Rq / 8, groups = 256 / cols;
   const int g = tid / cols, c = tid - g * cols;
   if (g < groups) {
@@ -114,8 +95,24 @@ __global__ __launch_bounds__(256) void paged_absorb_kernel(const PagedAttn a) {
   }
   for (int d = tid; d < a.Drp; d += 256)
     dst[2 * a.Rq + d] = d < a.Dr ? (bf16_t)(qp[d] ^ (a.neg ? 0x8000 : 0)) : bf16_t(0);
+  __syncthreads();   // the LDS is the next row's
 }
 
+// Tokens on the latent rows (at most).
+__device__ __forceinline__ int pg_tokens(const PagedAttn& a) {
+  return a.p.rows == a.p.offsets ? a.p.T : paged_clamp(a.p.rows[a.p.B], 0, a.p.T);
+}
+
+// A block takes (token, head) rows blockIdx.x, + gridDim.x, ..., head by head.  Thread
+// (g, c): columns 8 c .. 8 c + 7 over the D_nope rows g, g + groups, ..., the groups added
+// through LDS.
+__global__ __launch_bounds__(256) void paged_absorb_kernel(const PagedAttn a) {
+  const int tokens = pg_tokens(a);
+  for (int i = blockIdx.x; i < tokens * a.H; i += gridDim.x) {
+    const int h = i / tokens;
+    paged_absorb_row(a, i - h * tokens, h);
+  }
+}
 // One wave per (tile, key range), range fastest.  A range without keys writes nothing
 // (paged_out_kernel does not read it).  NS = Rq / 16; VEC: 16-byte loads of latent and
 // rope rows.
@@ -126,22 +123,21 @@ __global__ __launch_bounds__(256) void paged_few_kernel(const PagedAttn a) {
   extern __shared__ __attribute__((aligned(16))) char pg_tile[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int hi = lane >> 5, l32 = lane & 31;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
-  const int split = __builtin_amdgcn_readfirstlane((int)(unit % a.nsplit));
-  const int tnum = __builtin_amdgcn_readfirstlane((int)(unit / a.nsplit));
-  if (tnum >= a.tiles) return;
-  const PagedSeq s = paged_seq(a.p, paged_find(a.p, tnum, a.H, 32, 1));
-  if (s.b < 0) return;
-  const int M = s.n * a.H;
-  const int mt = tnum - (int)((int64_t)s.t0 * a.H / 32) - s.b;
-  if (32 * mt >= M) return;
+  const int units = ((int)((int64_t)pg_tokens(a) * a.H / 32) + a.p.B) * a.nsplit;
+  for (int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + wave); unit < units; unit += 4 * gridDim.x) {
+  const int tnum = unit / a.nsplit, split = unit - tnum * a.nsplit;
+  const PagedSeq s = paged_seq(a.p, paged_find(a.p, a.p.rows, tnum, a.H, 32, 1));
+  if (s.b < 0) continue;
+  const int M = s.m * a.H;
+  const int mt = tnum - (int)((int64_t)s.r0 * a.H / 32) - s.b;
+  if (32 * mt >= M) continue;
   const int kend = pg_kend(s, a.H, mt);
   const int kb = split * a.cpw * 32;
   const int ke = split == a.nsplit - 1 ? kend : min(kend, kb + a.cpw * 32);
-  if (kb >= ke) return;
+  if (kb >= ke) continue;
   const int row = 32 * mt + l32, rowc = min(row, M - 1);
   const int qpos = s.first + rowc / a.H;
-  const int64_t grow = (int64_t)s.t0 * a.H + rowc;
+  const int64_t grow = (int64_t)s.r0 * a.H + rowc;
   char* tile = pg_tile + wave * 32 * RB;
   const MlbLane<RB> lk(lane);
   const bf16_t* qrow = a.qabs + grow * (2 * a.Rq + a.Drp) + 8 * hi;
@@ -264,7 +260,7 @@ __global__ __launch_bounds__(256) void paged_few_kernel(const PagedAttn a) {
     asm volatile("" ::: "memory");
   }
   l = mla_pair_sum(l);
-  if (row >= M) return;
+  if (row >= M) continue;
   const int64_t part = (int64_t)split * a.p.T * a.H + grow;
   if (hi == 0) a.ml[part] = make_float2(m, l);
   float* po = a.po + part * a.Rq;
@@ -274,24 +270,25 @@ __global__ __launch_bounds__(256) void paged_few_kernel(const PagedAttn a) {
     for (int g = 0; g < 4; ++g)
       *reinterpret_cast<float4*>(po + 32 * v + 8 * g + 4 * hi) =
           make_float4(o[v][4 * g], o[v][4 * g + 1], o[v][4 * g + 2], o[v][4 * g + 3]);
+  }
 }
 
 // The ranges of a row added by their weights.  Every range that paged_few_kernel wrote
 // takes part, so a NaN in its sums reaches the output also through a weight of 0.  A
 // row that saw no key gives zeros.
-// Grid (T, H).  LDS (floats): weights of the ranges [PG_MAX_SPLITS] | group sums
+// Rows as paged_absorb_kernel takes them.  LDS (floats): weights of the ranges [PG_MAX_SPLITS] | group sums
 // [groups][Rq] (the first row then holds the normalised sum).
-__global__ __launch_bounds__(256) void paged_out_kernel(const PagedAttn a) {
+__device__ __forceinline__ void paged_out_row(const PagedAttn& a, int rt, int h) {
   extern __shared__ __attribute__((aligned(16))) float pg_sm[];
   float* wt = pg_sm;
   float* sum = pg_sm + PG_MAX_SPLITS;
-  const int tid = threadIdx.x, t = blockIdx.x, h = blockIdx.y;
-  const PagedSeq s = paged_seq(a.p, paged_find(a.p, t, 1, 1, 0));
-  const int i0 = t - s.t0;
-  if (s.b < 0 || i0 >= s.n) return;   // rows behind the last sequence stay as they were
-  const int64_t rows = (int64_t)a.p.T * a.H, p0 = (int64_t)t * a.H + h;
+  const int tid = threadIdx.x;
+  const PagedSeq s = paged_seq(a.p, paged_find(a.p, a.p.rows, rt, 1, 1, 0));
+  const int i0 = rt - s.r0;
+  if (s.b < 0 || i0 >= s.m) return;
+  const int64_t rows = (int64_t)a.p.T * a.H, p0 = (int64_t)rt * a.H + h;
   const int nr = pg_ranges(a, pg_kend(s, a.H, (i0 * a.H + h) / 32));
-  bf16_t* orow = a.out + p0 * a.Dv;
+  bf16_t* orow = a.out + ((int64_t)(s.t0 + i0) * a.H + h) * a.Dv;
   if (nr == 0) {
     for (int dv = tid; dv < a.Dv; dv += 256) orow[dv] = bf16_t(0);
     return;
@@ -370,6 +367,15 @@ __global__ __launch_bounds__(256) void paged_out_kernel(const PagedAttn a) {
   }
 }
 
+__global__ __launch_bounds__(256) void paged_out_kernel(const PagedAttn a) {
+  const int tokens = pg_tokens(a);   // rows behind the last sequence stay as they were
+  for (int i = blockIdx.x; i < tokens * a.H; i += gridDim.x) {
+    const int h = i / tokens;
+    if (i >= (int)gridDim.x) __syncthreads();   // the LDS is the last row's
+    paged_out_row(a, i - h * tokens, h);
+  }
+}
+
 // ------------------------------------------------------------------ host
 static int pg_validate(const dsmoe_mla_paged_dims* d) {
   const int rc = paged_validate(d);
@@ -384,7 +390,16 @@ static int pg_validate(const dsmoe_mla_paged_dims* d) {
   return DSMOE_OK;
 }
 
-static PagedAttn pg_args(const dsmoe_mla_paged_dims* d) {
+// More new tokens of a sequence than this have its K and V built (mla_paged_kv.hip):
+// for one (head, key) the latent rows cost 6 R + 2 D_rope operations a token (the two
+// parts of q_abs among them) against 2 (D_nope + D_rope + D_v), and K and V 2 R (D_nope + D_v) once.
+static int pg_threshold(const dsmoe_mla_paged_dims* d) {
+  const int64_t build = (int64_t)2 * d->R * (d->D_nope + d->D_v);
+  const int64_t more = 6 * d->R + 2 * d->D_rope - 2 * (d->D_nope + d->D_rope + d->D_v);
+  return more <= 0 ? INT_MAX : (int)std::max<int64_t>(16, build / more);
+}
+
+static PagedAttn pg_args(const dsmoe_mla_paged_dims* d, size_t* bytes, void* ws) {
   PagedAttn a;
   std::memset(static_cast<void*>(&a), 0, sizeof(a));
   a.p = paged_batch(d, nullptr, nullptr, nullptr);
@@ -392,32 +407,38 @@ static PagedAttn pg_args(const dsmoe_mla_paged_dims* d) {
   for (int ns : {2, 4, 8, 12, 16})
     if (a.Rq == 0 && d->R <= 16 * ns) a.Rq = 16 * ns;
   a.Drp = (int)align_up(d->D_rope, 16);
-  a.tiles = (int)((int64_t)d->T * d->H / 32) + d->B;
-  // about 1024 waves (four for each CU) if every sequence were as long as the longest
-  const int64_t chunks = std::max<int64_t>(1, cdiv(d->max_kv, 32));
-  const int64_t tiles = std::max<int64_t>(1, cdiv((int64_t)d->T * d->H, 32));
-  a.cpw = (int)std::max<int64_t>(std::max<int64_t>(1, tiles * chunks / 1024), cdiv(chunks, PG_MAX_SPLITS));
-  a.nsplit = (int)cdiv(chunks, a.cpw);
   a.neg = d->softmax_scale < 0.0f ? 1 : 0;
   // not below the smallest normal number: a masked score, -infinity, stays one for a scale of 0
   a.c = std::max((d->softmax_scale < 0.0f ? -d->softmax_scale : d->softmax_scale) * MLA_LOG2E, FLT_MIN);
-  return a;
-}
-
-static size_t pg_carve(PagedAttn& a, void* ws) {
   Carver c(ws);
+  a.thr = pg_threshold(d);
+  // with longer chunks about, most of the tokens are theirs: as many row tiles here as
+  // every sequence has for one token
   const size_t rows = (size_t)a.p.T * a.H;
+  const bool both = d->max_q > a.thr && paged_kv_carve(a, d, c) > 0;
+  if (!both) a.slots = 0;
+  const int64_t tiles = std::max<int64_t>(1, cdiv(both ? (int64_t)d->B * d->H : (int64_t)rows, 32));
+  // about 1024 waves (four for each CU) if every sequence were as long as the longest
+  const int64_t chunks = std::max<int64_t>(1, cdiv(d->max_kv, 32));
+  a.cpw = (int)std::max<int64_t>(std::max<int64_t>(1, tiles * chunks / 1024), cdiv(chunks, PG_MAX_SPLITS));
+  // the partial sums of all rows in 256 MB, or one range
+  const int64_t most = std::max<int64_t>(1, (int64_t(256) << 20) / std::max<int64_t>(1, (int64_t)rows * a.Rq * 4));
+  a.cpw = (int)std::max<int64_t>(a.cpw, cdiv(chunks, most));
+  a.nsplit = (int)cdiv(chunks, a.cpw);
   a.qabs = c.take<bf16_t>(rows * (2 * a.Rq + a.Drp));
   a.ml = c.take<float2>(rows * a.nsplit);
   a.po = c.take<float>(rows * a.nsplit * a.Rq);
-  return c.used();
+  *bytes = c.used();
+  return a;
 }
 
 template <int NS>
-static int launch_paged_few(const PagedAttn& a, bool vec, hipStream_t st) {
+static int launch_paged_few(const PagedAttn& a, hipStream_t st) {
   constexpr size_t lds = 4 * 32 * ((NS * 16 + 127) / 128 * 256);
-  auto kern = vec ? paged_few_kernel<NS, true> : paged_few_kernel<NS, false>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)cdiv((int64_t)a.tiles * a.nsplit, 4)), dim3(256), lds, st, a);
+  auto kern = a.kvvec ? paged_few_kernel<NS, true> : paged_few_kernel<NS, false>;
+  int64_t blocks = cdiv(((int64_t)a.p.T * a.H / 32 + a.p.B) * a.nsplit, 4);
+  if (a.slots) blocks = std::min<int64_t>(blocks, 2048);
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, a);
   return check_launch("mla_paged_few");
 }
 
@@ -427,8 +448,9 @@ using namespace dsmoe;
 
 extern "C" size_t dsmoe_mla_attn_paged_workspace_size(const dsmoe_mla_paged_dims* dims) {
   if (pg_validate(dims)) return 0;
-  PagedAttn a = pg_args(dims);
-  return std::max<size_t>(pg_carve(a, nullptr), 256);
+  size_t need = 0;
+  pg_args(dims, &need, nullptr);
+  return std::max<size_t>(need, 256);
 }
 
 extern "C" int dsmoe_mla_attn_paged(const void* q_nope, const void* q_pe, const void* kv_pages, const void* pe_pages,
@@ -444,12 +466,11 @@ extern "C" int dsmoe_mla_attn_paged(const void* q_nope, const void* q_pe, const 
   DSMOE_REQUIRE(wk_head_stride >= 0 && wv_head_stride >= 0 && dims->qn_token_stride >= 0 && dims->qn_head_stride >= 0 &&
                     dims->qp_token_stride >= 0 && dims->qp_head_stride >= 0, DSMOE_ERR_INVALID,
                 "mla_paged: negative stride");
-  PagedAttn a = pg_args(dims);
-  const size_t need = pg_carve(a, nullptr);
+  size_t need = 0;
+  PagedAttn a = pg_args(dims, &need, workspace);
   DSMOE_REQUIRE(workspace && workspace_bytes >= need, DSMOE_ERR_WORKSPACE, "mla_paged: workspace too small");
   const auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   DSMOE_REQUIRE(al(workspace), DSMOE_ERR_INVALID, "mla_paged: workspace must be 16-byte aligned");
-  pg_carve(a, workspace);
   a.p = paged_batch(dims, block_table, kv_lens, q_offsets);
   a.q_nope = static_cast<const bf16_t*>(q_nope);
   a.q_pe = static_cast<const bf16_t*>(q_pe);
@@ -463,22 +484,33 @@ extern "C" int dsmoe_mla_attn_paged(const void* q_nope, const void* q_pe, const 
   a.wv_hs = wv_head_stride;
   a.out = static_cast<bf16_t*>(out);
   a.wvec = (a.R % 8 == 0 && wk_head_stride % 8 == 0 && wv_head_stride % 8 == 0 && al(wkv_b_k) && al(wkv_b_v)) ? 1 : 0;
-  const bool vec = a.R % 8 == 0 && a.Dr % 8 == 0 && a.p.kv_ps % 8 == 0 && a.p.kv_rs % 8 == 0 && a.p.pe_ps % 8 == 0 &&
-                   a.p.pe_rs % 8 == 0 && al(kv_pages) && al(pe_pages);
+  a.kvvec = (a.R % 8 == 0 && a.Dr % 8 == 0 && a.p.kv_ps % 8 == 0 && a.p.kv_rs % 8 == 0 && a.p.pe_ps % 8 == 0 &&
+             a.p.pe_rs % 8 == 0 && al(kv_pages) && al(pe_pages)) ? 1 : 0;
+  a.qvec = (a.Dn % 8 == 0 && a.Dr % 8 == 0 && a.qn_ts % 8 == 0 && a.qn_hs % 8 == 0 && a.qp_ts % 8 == 0 &&
+            a.qp_hs % 8 == 0 && al(q_nope) && al(q_pe)) ? 1 : 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)a.p.T, (unsigned)a.H);
-  hipLaunchKernelGGL(paged_absorb_kernel, grid, dim3(256), sizeof(float) * (256 / (a.Rq / 8)) * a.Rq, st, a);
+  int64_t blocks = (int64_t)a.p.T * a.H;
+  if (a.slots) {
+    rc = launch_paged_plan(a, st);
+    if (rc) return rc;
+    rc = launch_paged_kv(a, st);
+    if (rc) return rc;
+    a.p.rows = a.plan_rows;
+    // most of the tokens are not the latent rows': blocks that take several
+    blocks = std::min<int64_t>(blocks, 4096);
+  }
+  hipLaunchKernelGGL(paged_absorb_kernel, dim3((unsigned)blocks), dim3(256), sizeof(float) * (256 / (a.Rq / 8)) * a.Rq, st, a);
   rc = check_launch("mla_paged_absorb");
   if (rc) return rc;
   switch (a.Rq / 16) {
-    case 2: rc = launch_paged_few<2>(a, vec, st); break;
-    case 4: rc = launch_paged_few<4>(a, vec, st); break;
-    case 8: rc = launch_paged_few<8>(a, vec, st); break;
-    case 12: rc = launch_paged_few<12>(a, vec, st); break;
-    default: rc = launch_paged_few<16>(a, vec, st); break;
+    case 2: rc = launch_paged_few<2>(a, st); break;
+    case 4: rc = launch_paged_few<4>(a, st); break;
+    case 8: rc = launch_paged_few<8>(a, st); break;
+    case 12: rc = launch_paged_few<12>(a, st); break;
+    default: rc = launch_paged_few<16>(a, st); break;
   }
   if (rc) return rc;
-  hipLaunchKernelGGL(paged_out_kernel, grid, dim3(256),
+  hipLaunchKernelGGL(paged_out_kernel, dim3((unsigned)blocks), dim3(256),
                      sizeof(float) * (PG_MAX_SPLITS + (size_t)(256 / (a.Rq / 4)) * a.Rq), st, a);
   return check_launch("mla_paged_out");
 }

@@ -1,5 +1,5 @@
 // Types, swizzled LDS tiles and lane-pair reductions shared by the MLA attention
-// kernels (mla.hip, mla_few.hip).
+// kernels (mla.hip, mla_few.hip, mla_paged.hip, mla_paged_kv.hip).
 #pragma once
 
 #include "common.h"
@@ -75,6 +75,44 @@ __device__ __forceinline__ float mla_pair_max(float x) {
 __device__ __forceinline__ float mla_pair_sum(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
   return __int_as_float(r[0]) + __int_as_float(r[1]);
+}
+
+// ---------------------------------------------------------------- work items
+// The attention kernels' work items are (batch-head pair hb, rank) with rank
+// r the r-th longest of a pair's items under the causal mask (the forward
+// and dQ kernels: query blocks from the last; the dK, dV kernel: key blocks
+// from the first).  Block i runs on XCD i % 8 (local index j = i / 8).  With
+// at least MLA_SPREAD pairs, XCD x owns the pairs x, x + 8, ... (their K, V
+// or query-side rows share its L2) and walks them rank-major, so the
+// dispatcher, which starts blocks in order as slots free up, runs every
+// pair's longest item first and the short ones fill the tail.  Fewer pairs:
+// the XCDs take contiguous eighths of the pair-major list (every XCD busy).
+// Grid: 8 * ceil(BH / 8) * nrank blocks; false for a block past the items.
+constexpr int MLA_SPREAD = 32;
+
+__device__ __forceinline__ bool mla_item(int blk, int BH, int nrank, int& hb, int& rank) {
+  const int x = blk & 7, j = blk >> 3;
+  if (BH >= MLA_SPREAD) {
+    const int nh = (BH - x + 7) >> 3;   // pairs on this XCD
+    if (j >= nh * nrank) return false;
+    rank = j / nh;
+    hb = x + 8 * (j - rank * nh);
+    return true;
+  }
+  const int total = BH * nrank, per = (total + 7) / 8;
+  const int item = x * per + j;
+  if (j >= per || item >= total) return false;
+  hb = item / nrank;
+  rank = item - hb * nrank;
+  return true;
+}
+
+__host__ __device__ inline int64_t mla_grid(int BH, int nrank) { return 8 * (int64_t)((BH + 7) / 8) * nrank; }
+
+// The 8-byte unit swizzle of a staged V tile of 32 NV columns (mla_fa_kernel).
+template <int NV>
+__device__ __forceinline__ int mla_vswz(int k) {
+  return NV == 1 ? 0 : NV == 2 ? 8 * ((k >> 1) & 1) : 8 * (k & 3);
 }
 
 }  // namespace dsmoe

@@ -1,4 +1,4 @@
-"""The paged latent cache and its attention (csrc/mla_cache.hip, csrc/mla_paged.hip) against the float64 oracle.
+"""The paged latent cache and its attention (csrc/mla_cache.hip, csrc/mla_paged.hip, csrc/mla_paged_kv.hip) against the float64 oracle.
 
 Bounds, derived from the arithmetic.  Append: one rounding to bf16 (2^-8 of the value) behind fp32 arithmetic of R + 8
 roundings at most (2^-24 each).  Attention: the output's rounding (2^-8 of it), the probabilities' (2^-8 of
@@ -52,11 +52,12 @@ def _call(x, scale, **kw):
     return mla_attention_paged(*[x[k] for k in ORDER], scale, **kw)
 
 
-def _check(got, x, scale, built=False):
+def _check(got, x, scale):
     ref, spread, size = attend_ref(*[x[k] for k in ORDER], scale)
     rows = ~torch.isnan(ref).all(-1).all(-1)
     got = got.detach().cpu().double()
     Dn, R, Dr = x["q_nope"].shape[2], x["kv_pages"].shape[2], x["pe_pages"].shape[2]
+    built = int((x["offsets"][1:] - x["offsets"][:-1]).max()) > 16   # K and V are built for some sequence, maybe
     d = size * (2.0 ** -11 if built else 2.0 ** -16) + size * (Dn + 2 * R + Dr) * 2.0 ** -24
     bound = 2.0 ** -8 * ref.abs() + spread * (2.0 ** -8 + 2.0 ** -10 + torch.expm1(2 * d)[..., None]) + 1e-30
     off = (got - ref).abs()[rows]
@@ -86,15 +87,55 @@ def test_attention(new, kv, page, shape):
     _check(_call(_gpu(x), scale, max_q=max(new), max_kv=max(kv)), x, scale)
 
 
+@pytest.mark.parametrize("new,kv,page,shape", [
+    ([300], [300], 64, MID),                             # a fresh prompt, key ranges
+    ([500, 1, 47, 46, 0, 1], [1400, 900, 47, 300, 50, 1], 48, MID),   # chunks beside decoding sequences, both sides of the line
+    ([129, 200], [129, 1000], 16, WIDE),
+    ([1300], [2000], 128, WIDE),
+    ([33] * 70 + [1] * 5, [33 + 3 * i for i in range(75)], 16, SMALL),  # more sequences than lanes
+    ([64, 130, 17], [64, 131, 300], 37, ODD),            # element loads of queries, latent rows and weights
+    ([128], [128], 1, MID),                              # whole tiles
+    ([257], [513], 64, dict(MID, H=5)),
+    ([70, 60], [70, 161], 16, dict(H=2, R=250, Dn=200, Dr=50, Dv=250)),
+    ([200], [333], 16, dict(H=2, R=128, Dn=16, Dr=240, Dv=256)),
+    ([200, 150], [200, 400], 16, dict(H=40, R=64, Dn=32, Dr=16, Dv=32)),
+])
+def test_chunks(new, kv, page, shape):
+    x, scale = _batch(new, kv, page, seed=len(new) + kv[0], shape=shape)
+    _check(_call(_gpu(x), scale, max_q=max(new), max_kv=max(kv)), x, scale)
+    _check(_call(_gpu(x), scale), x, scale)
+
+
+def test_chunks_in_several_passes():
+    """K and V of one pass hold 4 GiB: a table far wider than the sequences are long."""
+    new = [129] * 8 + [1]
+    x, scale = _batch(new, [n + 40 for n in new], 64, seed=31, shape=WIDE, width=512)
+    _check(_call(_gpu(x), scale), x, scale)
+
+
+@pytest.mark.parametrize("c,pe,w", [(1e20, 1e20, 1e-10), (1e-20, 1e-20, 1e-10), (3e4, 1.0, 1e3), (1e-6, 1e6, 1.0)])
+def test_magnitudes_past_half_precision(c, pe, w):
+    """Keys, values, queries far above and below what 16-bit floats of five exponent bits hold, in one batch with ordinary ones."""
+    x, scale = _batch([150, 100, 3], [150, 333, 90], 16, seed=33, shape=MID)
+    lo = x["kv_pages"].shape[0] // 2
+    x["kv_pages"][:lo] = (x["kv_pages"][:lo].float() * c).bfloat16()
+    x["pe_pages"][:lo] = (x["pe_pages"][:lo].float() * pe).bfloat16()
+    x["w_k"], x["w_v"] = (x["w_k"].float() * w).bfloat16(), (x["w_v"].float() * w).bfloat16()
+    z = max(1.0, c * w, pe)
+    x["q_nope"], x["q_pe"] = (x["q_nope"].float() / z).bfloat16(), (x["q_pe"].float() / z).bfloat16()
+    _check(_call(_gpu(x), scale), x, scale)
+
+
 @pytest.mark.parametrize("scale", [-0.3, 2.0, 0.0])
-def test_scales(scale):
-    x, _ = _batch([1, 6], [200, 90], 16, seed=3, shape=SMALL)
+@pytest.mark.parametrize("n", [6, 60])
+def test_scales(scale, n):
+    x, _ = _batch([1, n], [200, 90], 16, seed=3, shape=SMALL)
     _check(_call(_gpu(x), scale), x, scale)
 
 
 def test_hints_do_not_change_what_is_computed():
     """max_q and max_kv far too small or large: every position and token still counts."""
-    x, scale = _batch([1, 20, 3], [900, 400, 64], 16, seed=5, shape=MID)
+    x, scale = _batch([1, 60, 3], [900, 400, 64], 16, seed=5, shape=MID)
     g = _gpu(x)
     for kw in (dict(), dict(max_q=1, max_kv=1), dict(max_q=0, max_kv=0), dict(max_q=10 ** 6, max_kv=2 ** 40)):
         _check(_call(g, scale, **kw), x, scale)
@@ -145,8 +186,9 @@ def test_rows_without_anything():
     assert (_call(y, scale, out=out.fill_(3.0)) == 3.0).all()
 
 
-def test_pages_that_are_not_there_and_lengths_past_the_table():
-    x, scale = _batch([2, 5, 1], [100, 90, 60], 16, seed=11, shape=MID)
+@pytest.mark.parametrize("n", [5, 55])
+def test_pages_that_are_not_there_and_lengths_past_the_table(n):
+    x, scale = _batch([2, n, 1], [100, 90, 60], 16, seed=11, shape=MID)
     x["table"][0, 2] = -1
     x["table"][1, 0] = 10 ** 6
     x["table"][1, 5] = x["kv_pages"].shape[0]
@@ -156,37 +198,40 @@ def test_pages_that_are_not_there_and_lengths_past_the_table():
     x["kv_lens"][0] = 2 ** 31 - 1
     got = _call(_gpu(x), scale)
     _check(got, x, scale)
-    assert (got[7] == 0).all()                       # a sequence without a single page
+    assert (got[n + 2] == 0).all()                   # a sequence without a single page
 
 
 def test_offsets_that_are_out_of_range_stay_inside():
     """Offsets past T, or decreasing ones: clamped, the sound sequences unharmed."""
-    x, scale = _batch([2, 3], [30, 40], 16, seed=12, shape=SMALL)
-    clean = _call(_gpu(x), scale)
-    x["offsets"] = torch.tensor([0, 2, 10 ** 9], dtype=torch.int32)
-    x["kv_lens"][1] = 40
-    assert torch.equal(_call(_gpu(x), scale), clean)
-    x["offsets"] = torch.tensor([0, 2, -5], dtype=torch.int32)
-    assert torch.equal(_call(_gpu(x), scale)[:2], clean[:2])
+    for n in (3, 53):
+        x, scale = _batch([2, n], [30, 60], 16, seed=12, shape=SMALL)
+        clean = _call(_gpu(x), scale)
+        x["offsets"] = torch.tensor([0, 2, 10 ** 9], dtype=torch.int32)
+        assert torch.equal(_call(_gpu(x), scale), clean)
+        x["offsets"] = torch.tensor([0, 2, -5], dtype=torch.int32)
+        assert torch.equal(_call(_gpu(x), scale)[:2], clean[:2])
+        x["offsets"] = torch.tensor([-9, 2, 2 + n], dtype=torch.int32)
+        assert torch.equal(_call(_gpu(x), scale), clean)
 
 
 @pytest.mark.parametrize("what", [float("nan"), float("inf"), float("-inf")])
-def test_not_finite_rows_reach_those_that_see_them(what):
+@pytest.mark.parametrize("n", [9, 150])
+def test_not_finite_rows_reach_those_that_see_them(what, n):
     """In a cached row: NaN in the tokens that see it, the others' bits unchanged; behind a sequence's length, on unused
     pages and in another sequence: nothing."""
-    x, scale = _batch([9, 1, 4], [60, 200, 4], 16, seed=13, shape=SMALL)
+    x, scale = _batch([n, 1, 4], [n + 51, 200, 4], 16, seed=13, shape=SMALL)
     g = _gpu(x)
     clean = _call(g, scale)
-    for j in (0, 30, 52, 55, 59):                    # sequence 0's new tokens stand at 51 .. 59
+    for j in (0, 30, 52, 55, n + 43, n + 50):        # sequence 0's new tokens stand at 51 .. n + 50
         bad = dict(g, kv_pages=g["kv_pages"].clone())
         bad["kv_pages"][int(x["table"][0, j // 16]), j % 16, 3] = what
         got = _call(bad, scale)
-        sees = torch.arange(14, device=DEV) + 51 >= j
-        sees[9:] = False
+        sees = torch.arange(n + 5, device=DEV) + 51 >= j
+        sees[n:] = False
         assert torch.isnan(got[sees]).any(-1).all() and torch.equal(got[~sees], clean[~sees]), j
     used = torch.zeros(g["kv_pages"].shape[:2], dtype=torch.bool)
-    for b, n in enumerate((60, 200, 4)):
-        for j in range(n):
+    for b, kv in enumerate((n + 51, 200, 4)):
+        for j in range(kv):
             used[int(x["table"][b, j // 16]), j % 16] = True
     bad = dict(g, kv_pages=g["kv_pages"].clone(), pe_pages=g["pe_pages"].clone())
     bad["kv_pages"][~used.to(DEV)] = what
@@ -269,10 +314,10 @@ def test_a_prompt_in_chunks_is_the_contiguous_attention(chunks):
 def test_captured_calls_replay_on_other_lengths_pages_and_values():
     """append and attend in a graph; between replays eager calls of the same operators on the same stream."""
     from dsmoe.mla import mla_cache_append
-    x, scale = _batch([4, 1, 0], [70, 40, 64], 16, seed=21, shape=MID)
+    x, scale = _batch([4, 61, 0], [70, 70, 64], 16, seed=21, shape=MID)
     g = _gpu(x)
-    c, pe = torch.randn(5, 192, device=DEV).bfloat16(), torch.randn(5, 24, device=DEV).bfloat16()
-    out = torch.empty(5, 12, 64, dtype=torch.bfloat16, device=DEV)
+    c, pe = torch.randn(65, 192, device=DEV).bfloat16(), torch.randn(65, 24, device=DEV).bfloat16()
+    out = torch.empty(65, 12, 64, dtype=torch.bfloat16, device=DEV)
 
     def step(x, c, pe, out):
         mla_cache_append(c, pe, x["kv_pages"], x["pe_pages"], x["table"], x["kv_lens"], x["offsets"])
@@ -282,7 +327,7 @@ def test_captured_calls_replay_on_other_lengths_pages_and_values():
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         step(g, c, pe, out)
-    for new, kv in (([4, 1, 0], [70, 40, 64]), ([1, 1, 3], [9, 71, 30]), ([0, 5, 0], [1, 48, 2])):
+    for new, kv in (([4, 61, 0], [70, 70, 64]), ([1, 1, 63], [9, 71, 64]), ([0, 65, 0], [1, 68, 2]), ([22, 21, 22], [40, 40, 30])):
         g["kv_lens"].copy_(torch.tensor(kv))
         g["offsets"].copy_(torch.tensor([0, *new]).cumsum(0))
         g["table"].copy_(g["table"].flip(1) if new[0] == 1 else g["table"])
@@ -295,8 +340,8 @@ def test_captured_calls_replay_on_other_lengths_pages_and_values():
 
 
 def test_two_streams_at_once():
-    x, scale = _batch([3, 1], [300, 700], 16, seed=23, shape=MID)
-    y, _ = _batch([1, 1], [900, 33], 16, seed=24, shape=MID)
+    x, scale = _batch([3, 100], [300, 700], 16, seed=23, shape=MID)
+    y, _ = _batch([70, 1], [900, 33], 16, seed=24, shape=MID)
     a, b = _gpu(x), _gpu(y)
     want = _call(a, scale), _call(b, scale)
     torch.cuda.synchronize()
