@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void mla_cache_append_kernel(const CacheArgs a
       cache_ld8<T>(a.ctx_kv, t * a.ckv_rs + c8, v);
     if (a.norm_w && !pe_side) cache_ld8<float>(a.norm_w, c8, w);
   }
-  const PagedSeq s = paged_seq(a.p, paged_find(a.p, a.p.offsets, t, 1, 1, 0));
+  const PagedSeq s = paged_at<PAGED_OFFSETS>(a.p, t, 1, 1, 0);
   const int pos = s.first + t - s.t0;
   // rows behind the last sequence, and positions without a place, are left alone
   if (s.b < 0 || t - s.t0 >= s.n || pos < 0 || pos >= s.kv) return;
@@ -109,6 +109,8 @@ int paged_validate(const dsmoe_mla_paged_dims* d) {
                 "mla_paged: R and D_rope must be in 1 .. 256");
   DSMOE_REQUIRE(d->pages > 0 && d->page_size > 0 && d->table_width >= 0, DSMOE_ERR_INVALID,
                 "mla_paged: pages and page_size must be positive");
+  DSMOE_REQUIRE((int64_t)d->table_width * d->page_size < (int64_t(1) << 31) - (1 << 16), DSMOE_ERR_UNSUPPORTED,
+                "mla_paged: a row of the table has room for 2^31 positions");
   DSMOE_REQUIRE(d->table_stride >= 0 && d->kv_page_stride >= 0 && d->kv_row_stride >= 0 && d->pe_page_stride >= 0 &&
                     d->pe_row_stride >= 0, DSMOE_ERR_INVALID, "mla_paged: negative stride");
   return DSMOE_OK;
@@ -118,10 +120,12 @@ PagedBatch paged_batch(const dsmoe_mla_paged_dims* d, const int32_t* table, cons
                        const int32_t* offsets) {
   PagedBatch p;
   p.table = table; p.kv_lens = kv_lens; p.offsets = p.rows = offsets;
+  p.units = nullptr;
   p.table_stride = d->table_stride;
   p.kv_ps = d->kv_page_stride; p.kv_rs = d->kv_row_stride;
   p.pe_ps = d->pe_page_stride; p.pe_rs = d->pe_row_stride;
   p.T = d->T; p.B = d->B; p.pages = d->pages; p.page_size = d->page_size; p.width = d->table_width;
+  p.page_shift = (p.page_size & (p.page_size - 1)) == 0 ? __builtin_ctz(p.page_size) : -1;
   return p;
 }
 

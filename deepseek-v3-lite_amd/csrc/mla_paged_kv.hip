@@ -19,7 +19,7 @@
 // their V rows, the row's own for q.  They return where a scalar costs nothing: kx and
 // q's in the factor of the scores, vx as weight 2^vx in the softmax,
 //   out = sum_j 2^(s_j + vx_j - m) (2^-vx_j v_j) / sum_j 2^(s_j + vx_j - m) 2^-vx_j,
-// m the running maximum of s_j + vx_j, so p stays at most 1.
+// m the running maximum of s_j + vx_j, or one up to 2^8 behind it.
 //
 // Masked places: a key on no page has its bit in `gone` (and zero rows); a latent row
 // with a NaN or an infinity has K all NaN and V zero, so that it reaches the queries that
@@ -41,6 +41,7 @@ constexpr int PKV_KB = 64;      // keys of a block of the attention
 __global__ __launch_bounds__(64) void paged_plan_kernel(const PagedAttn a) {
   const int lane = threadIdx.x;
   int slot0 = 0, row0 = 0;
+  PagedUnits units;
   for (int b0 = 0; b0 < a.p.B; b0 += 64) {
     const int b = b0 + lane;
     PagedSeq s = paged_seq(a.p, min(b, a.p.B - 1));
@@ -63,9 +64,13 @@ __global__ __launch_bounds__(64) void paged_plan_kernel(const PagedAttn a) {
       if (has) a.seq_of[slot] = b;
       a.plan_rows[b] = (int)min((int64_t)a.p.T, row0 + sum - own);
     }
+    // (of sane offsets the sum stays under T; others' tokens behind it are left out)
+    const int m = (int)(min((int64_t)a.p.T, row0 + sum) - min((int64_t)a.p.T, row0 + sum - own));
+    paged_unit_step(a, b, m, s.kv, units);
     row0 = (int)min((int64_t)a.p.T, row0 + __shfl(sum, 63));
   }
   if (lane == 0) a.plan_rows[a.p.B] = row0;
+  paged_unit_end(a, units);
   for (int i = min(slot0, a.slots) + lane; i < a.slots; i += 64) a.seq_of[i] = -1;
 }
 
@@ -94,136 +99,178 @@ __device__ __forceinline__ uint32_t pkv_pack(float a, float b) {
   return __builtin_bit_cast(uint32_t, v);
 }
 
-// Grid (cap / 128, H, slots of the pass).  VPART: V, else K.  NT: 32-column tiles, all
-// computed (weight rows past the last one repeat it and are not stored).  VEC: 16-byte
-// loads of latent, rope and weight rows, every load of a batch issued from a valid
+// Grid (tiles of 128 positions / a.kvt, H, slots of the pass).  A block keeps its head's weight
+// rows in LDS (mlb_off layout) for a.kvt tiles, whose latent rows are asked for one tile
+// ahead: read by every wave from memory they took 232 us for two prompts of 6144 positions (H 32,
+// R 256, D_nope and D_v 128), this way XXX us.  part: K, V, or 2: by the block's parity.  NT: 32-column tiles,
+// all computed (LDS rows past the last weight row repeat it and are not stored).  VEC:
+// 16-byte loads of latent, rope and weight rows, every load of a batch issued from a valid
 // address before it is used.
-template <int NS, int NT, bool VEC, bool VPART>
-__global__ __launch_bounds__(256) void paged_kv_kernel(const PagedAttn a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+template <int NS, int NT, bool VEC>
+__global__ __launch_bounds__(256) void paged_kv_kernel(const PagedAttn a, int part) {
+  constexpr int RB = (NS * 16 + 127) / 128 * 256;
+  extern __shared__ __attribute__((aligned(16))) char pkv_smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hi = lane >> 5, l32 = lane & 31;
-  const int h = blockIdx.y, slot = blockIdx.z;
+  const int h = blockIdx.y, slot = part == 2 ? blockIdx.z >> 1 : blockIdx.z;
+  const bool vpart = part == 2 ? blockIdx.z & 1 : part;
   const PagedSeq s = paged_seq(a.p, a.seq_of[a.slot0 + slot]);
-  const int k0 = blockIdx.x * PKV_ROWS + 32 * wave;
-  if (s.b < 0 || (int)blockIdx.x * PKV_ROWS >= s.kv) return;
-  const int ncols = VPART ? a.Dv : a.Dn;
-  const int64_t sh = (int64_t)slot * a.H + h, meta = sh * (a.cap / 32) + k0 / 32;
-  const int key = k0 + l32;
-  int in_page;
-  const int page = paged_page(a.p, s.b, min(key, s.kv - 1), in_page);
-  const bool live = key < s.kv && page >= 0;
-  const int64_t pg = max(page, 0);
-  const bf16_t* cr = a.kv_pages + pg * a.p.kv_ps + in_page * a.p.kv_rs;
-  const bf16_t* pr = a.pe_pages + pg * a.p.pe_ps + in_page * a.p.pe_rs;
-  const bf16_t* w = VPART ? a.w_v + h * a.wv_hs : a.w_k + h * a.wk_hs;
+  const int tile0 = blockIdx.x * a.kvt, tiles = min(tile0 + a.kvt, (s.kv + PKV_ROWS - 1) / PKV_ROWS);
+  if (s.b < 0 || tile0 >= tiles) return;
+  const int ncols = vpart ? a.Dv : a.Dn;
+  const int64_t sh = (int64_t)slot * a.H + h;
+  const bf16_t* w = vpart ? a.w_v + h * a.wv_hs : a.w_k + h * a.wk_hs;
+  // the lane's latent and rope row of a tile; positions behind the last one read that
   bf16x8_t fx[NS];
-#pragma unroll
-  for (int st = 0; st < NS; ++st) {
-    const int col = 16 * st + 8 * hi;
-    mla_u32x4 v = pkv_ld8(cr + (VEC ? min(col, a.R - 8) : col), a.R - col, VEC);
-    if (col >= a.R) v = mla_u32x4{0u, 0u, 0u, 0u};
-    fx[st] = __builtin_bit_cast(bf16x8_t, v);
-  }
-  mla_f32x16 acc[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const bf16_t* wr = w + (int64_t)min(32 * j + l32, ncols - 1) * a.R;
-    bf16x8_t fw[NS];
+  const bf16_t* pr;
+  int page, in_page, npage, nin_page;
+  bool live, gone1;
+  const auto key_of = [&](int t) { return t * PKV_ROWS + 32 * wave + l32; };
+  const auto lookup = [&](int t) { npage = paged_page(a.p, s.b, min(key_of(t), s.kv - 1), nin_page); };
+  const auto load = [&](int t) {
+    live = key_of(t) < s.kv && page >= 0;
+    gone1 = key_of(t) < s.kv && page < 0;
+    const int64_t pg = max(page, 0);
+    const bf16_t* cr = a.kv_pages + pg * a.p.kv_ps + in_page * a.p.kv_rs;
+    pr = a.pe_pages + pg * a.p.pe_ps + in_page * a.p.pe_rs;
 #pragma unroll
     for (int st = 0; st < NS; ++st) {
       const int col = 16 * st + 8 * hi;
-      fw[st] = __builtin_bit_cast(bf16x8_t, pkv_ld8(wr + (VEC ? min(col, a.R - 8) : col), a.R - col, VEC));
+      fx[st] = __builtin_bit_cast(bf16x8_t, pkv_ld8(cr + (VEC ? min(col, a.R - 8) : col), a.R - col, VEC));
     }
+  };
+  lookup(tile0);
+  page = npage;
+  in_page = nin_page;
+  // the weight rows, each thread's pieces in a batch
+  {
+    constexpr int PER = (NT * 32 * NS * 2 + 255) / 256;
+    mla_u32x4 v[PER];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[j][i] = 0.0f;
+    for (int u = 0; u < PER; ++u) {
+      const int i = tid + 256 * u, r = i / (2 * NS), c = i - r * (2 * NS);
+      v[u] = pkv_ld8(w + (int64_t)min(r, ncols - 1) * a.R + (VEC ? min(8 * c, a.R - 8) : 8 * c), a.R - 8 * c, VEC);
+    }
+    load(tile0);
+    lookup(tile0 + 1);
 #pragma unroll
-    for (int st = 0; st < NS; ++st)
-      acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fw[st], fx[st], acc[j], 0, 0, 0);
+    for (int u = 0; u < PER; ++u) {
+      const int i = tid + 256 * u, r = i / (2 * NS), c = i - r * (2 * NS);
+      if (i < NT * 32 * NS * 2) *reinterpret_cast<mla_u32x4*>(pkv_smem + mlb_off(r, c, RB)) = v[u];
+    }
   }
-  uint32_t nf = 0;
+  __syncthreads();
+  const MlbLane<RB> lk(lane);
+  for (int t = tile0; t < tiles; ++t) {
+    const int key = key_of(t);
+    uint32_t nf = 0;
 #pragma unroll
-  for (int st = 0; st < NS; ++st) nf = pkv_absmax(__builtin_bit_cast(mla_u32x4, fx[st]), nf);
-  const uint64_t bl = __builtin_amdgcn_ballot_w64(nf >= 0x7f800000u);
-  const bool bad = (((uint32_t)bl | (uint32_t)(bl >> 32)) >> l32) & 1;
-  // the largest finite magnitude of the wave's keys goes to [2^13, 2^14)
-  float mx = 0.0f;
+    for (int st = 0; st < NS; ++st) {
+      if (16 * st + 8 * hi >= a.R) fx[st] = __builtin_bit_cast(bf16x8_t, mla_u32x4{0u, 0u, 0u, 0u});
+      nf = pkv_absmax(__builtin_bit_cast(mla_u32x4, fx[st]), nf);
+    }
+    const uint64_t bl = __builtin_amdgcn_ballot_w64(nf >= 0x7f800000u);
+    const bool bad = (((uint32_t)bl | (uint32_t)(bl >> 32)) >> l32) & 1;
+    mla_f32x16 acc[NT];
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < NT; ++j) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(acc[j][i]));
-  if (!VPART)
-    for (int d = 8 * hi; d < a.Dr; d += 16) {
-      const mla_u32x4 v = pkv_ld8(pr + d, a.Dr - d, VEC);
+      for (int i = 0; i < 16; ++i) acc[j][i] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = fabsf(__uint_as_float(v[i] << 16)), y = fabsf(__uint_as_float(v[i] & 0xffff0000u));
-        mx = fmaxf(mx, x < INFINITY ? x : 0.0f);
-        mx = fmaxf(mx, y < INFINITY ? y : 0.0f);
+      for (int st = 0; st < NS; ++st)
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lk.frag(pkv_smem, 32 * j, st), fx[st], acc[j], 0, 0, 0);
+    }
+    const bool alive = live;
+    const uint32_t gone = (uint32_t)__builtin_amdgcn_ballot_w64(gone1);
+    const bf16_t* prow = pr;
+    if (t + 1 < tiles) {
+      page = npage;
+      in_page = nin_page;
+      lookup(t + 2);
+      __builtin_amdgcn_sched_barrier(0);   // (asked for before the rows: see paged_few_kernel)
+      load(t + 1);
+    }
+    // the largest finite magnitude of the wave's keys goes to [2^13, 2^14)
+    float mx = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(acc[j][i]));
+    if (!vpart)
+      for (int d = 8 * hi; d < a.Dr; d += 16) {
+        const mla_u32x4 v = pkv_ld8(prow + d, a.Dr - d, VEC);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = fabsf(__uint_as_float(v[i] << 16)), y = fabsf(__uint_as_float(v[i] & 0xffff0000u));
+          mx = fmaxf(mx, x < INFINITY ? x : 0.0f);
+          mx = fmaxf(mx, y < INFINITY ? y : 0.0f);
+        }
+      }
+    if (!alive || bad) mx = 0.0f;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
+    const int n = mx > 0.0f ? min(max(13 - ((int)(__float_as_uint(mx) >> 23) - 127), -126), 126) : 0;
+    if (lane == 0) {
+      const int64_t meta = sh * (a.cap / 32) + t * (PKV_ROWS / 32) + wave;
+      if (vpart) {
+        a.vx[meta] = (float)-n;
+      } else {
+        a.kx[meta] = pkv_pow2(-n);
+        a.gone[meta] = gone;
       }
     }
-  if (!live || bad) mx = 0.0f;
+    const float nan = __builtin_nanf("");
+    const bool zero = !alive || (vpart && bad);
+    // dead rows: zeros (a select: their values may be anything), NaN for K rows that hold one
+    const float f = pkv_pow2(n);
+    const auto put = [&](float v) { return zero ? 0.0f : (!vpart && bad) ? nan : v * f; };
+    _Float16* row = vpart ? a.vbuf + (sh * a.cap + key) * a.DVp : a.kbuf + (sh * a.cap + key) * a.DQp;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
-  const int n = mx > 0.0f ? min(max(13 - ((int)(__float_as_uint(mx) >> 23) - 127), -126), 126) : 0;
-  const uint32_t gone = (uint32_t)__builtin_amdgcn_ballot_w64(key < s.kv && page < 0);
-  if (lane == 0) {
-    if (VPART) {
-      a.vx[meta] = (float)-n;
-    } else {
-      a.kx[meta] = pkv_pow2(-n);
-      a.gone[meta] = gone;
-    }
-  }
-  float f = pkv_pow2(n);
-  const float nan = __builtin_nanf("");
-  _Float16* row = VPART ? a.vbuf + (sh * a.cap + key) * a.DVp : a.kbuf + (sh * a.cap + key) * a.DQp;
-  const bool zero = !live || (VPART && bad), isnan = !VPART && live && bad;
-  const auto put = [&](float v) { return isnan ? nan : zero ? 0.0f : v * f; };
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
+      for (int gp = 0; gp < 2; ++gp) {
+        // columns 32 j + 16 gp + 8 hi .. + 7 of the lane's key: the halves of a register
+        // pair (four columns each of lanes l and l + 32) change places
+        uint32_t u[2][2];
 #pragma unroll
-    for (int gp = 0; gp < 2; ++gp) {
-      // columns 32 j + 16 gp + 8 hi .. + 7 of the lane's key: the halves of a register
-      // pair (four columns each of lanes l and l + 32) change places
-      uint32_t u[2][2];
+        for (int g = 0; g < 2; ++g)
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
+          for (int d = 0; d < 2; ++d)
+            u[g][d] = pkv_pack(put(acc[j][8 * gp + 4 * g + 2 * d]), put(acc[j][8 * gp + 4 * g + 2 * d + 1]));
+        const auto r0 = __builtin_amdgcn_permlane32_swap(u[0][0], u[1][0], false, false);
+        const auto r1 = __builtin_amdgcn_permlane32_swap(u[0][1], u[1][1], false, false);
+        const int col = 32 * j + 16 * gp + 8 * hi;
+        const mla_u32x4 o = {(uint32_t)r0[0], (uint32_t)r1[0], (uint32_t)r0[1], (uint32_t)r1[1]};
+        if (col + 8 <= ncols) {
+          *reinterpret_cast<mla_u32x4*>(row + col) = o;
+        } else {
+          const f16x8_t e8 = __builtin_bit_cast(f16x8_t, o);
 #pragma unroll
-        for (int d = 0; d < 2; ++d)
-          u[g][d] = pkv_pack(put(acc[j][8 * gp + 4 * g + 2 * d]), put(acc[j][8 * gp + 4 * g + 2 * d + 1]));
-      const auto r0 = __builtin_amdgcn_permlane32_swap(u[0][0], u[1][0], false, false);
-      const auto r1 = __builtin_amdgcn_permlane32_swap(u[0][1], u[1][1], false, false);
-      const int col = 32 * j + 16 * gp + 8 * hi;
-      const mla_u32x4 o = {(uint32_t)r0[0], (uint32_t)r1[0], (uint32_t)r0[1], (uint32_t)r1[1]};
-      if (col + 8 <= ncols) {
-        *reinterpret_cast<mla_u32x4*>(row + col) = o;
+          for (int e = 0; e < 8; ++e)
+            if (col + e < ncols) row[col + e] = e8[e];
+        }
+      }
+    if (vpart) continue;
+    for (int d = 8 * hi; d < a.Dr; d += 16) {
+      const mla_u32x4 v = pkv_ld8(prow + d, a.Dr - d, VEC);
+      mla_u32x4 o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = __uint_as_float(v[i] << 16), y = __uint_as_float(v[i] & 0xffff0000u);
+        o[i] = alive ? pkv_pack(x * f, y * f) : 0u;
+      }
+      if (VEC && a.Dn % 8 == 0) {
+        *reinterpret_cast<mla_u32x4*>(row + a.Dn + d) = o;
       } else {
         const f16x8_t e8 = __builtin_bit_cast(f16x8_t, o);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (col + e < ncols) row[col + e] = e8[e];
+          if (d + e < a.Dr) row[a.Dn + d + e] = e8[e];
       }
     }
-  if (VPART) return;
-  if (!live) f = 0.0f;
-  for (int d = 8 * hi; d < a.Dr; d += 16) {
-    const mla_u32x4 v = pkv_ld8(pr + d, a.Dr - d, VEC);
-    mla_u32x4 o;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x = __uint_as_float(v[i] << 16), y = __uint_as_float(v[i] & 0xffff0000u);
-      o[i] = live ? pkv_pack(x * f, y * f) : 0u;
-    }
-    if (VEC && a.Dn % 8 == 0) {
-      *reinterpret_cast<mla_u32x4*>(row + a.Dn + d) = o;
-    } else {
-      const f16x8_t e8 = __builtin_bit_cast(f16x8_t, o);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (d + e < a.Dr) row[a.Dn + d + e] = e8[e];
-    }
+    for (int d = a.Dn + a.Dr + hi; d < a.DQp; d += 2) row[d] = (_Float16)0.0f;
   }
-  for (int d = a.Dn + a.Dr + hi; d < a.DQp; d += 2) row[d] = (_Float16)0.0f;
 }
 
 // ---------------------------------------------------------------- attention
@@ -238,11 +285,15 @@ struct PfaCfg {
   static constexpr int NLK = (KT / 1024 + NW - 1) / NW;  // 1 KB direct loads per wave and tile
   static constexpr int NLV = (VT / 1024 + NW - 1) / NW;
   static constexpr int QB = 32 * NW;
+  // two blocks of keys on their way where a third buffer leaves as many waves on a CU (and
+  // every wave has as many loads, which the waits count)
+  static constexpr bool EVEN = NLK * NW * 1024 == KT && NLV * NW * 1024 == VT;
+  static constexpr int NBUF = EVEN && 3 * BUF <= (NW == 8 ? 160 : 80) * 1024 ? 3 : 2;
 };
 
 // Query block tnum of the call: block numbers start at floor(offset / QB) + b.
 __device__ __forceinline__ bool pfa_block(const PagedAttn& a, int tnum, int QB, PagedSeq& s, int& slot, int& q0) {
-  s = paged_seq(a.p, paged_find(a.p, a.p.offsets, tnum, 1, QB, 1));
+  s = paged_at<PAGED_OFFSETS>(a.p, tnum, 1, QB, 1);
   if (s.b < 0) return false;
   slot = __builtin_amdgcn_readfirstlane(a.slot_of[s.b]) - a.slot0;
   q0 = (tnum - s.t0 / QB - s.b) * QB;
@@ -315,10 +366,10 @@ __global__ __launch_bounds__(64 * NW) void paged_fa_kernel(const PagedAttn a) {
   const char* kg = reinterpret_cast<const char*>(a.kbuf + sh * a.cap * C::DQp);
   const char* vg = reinterpret_cast<const char*>(a.vbuf + sh * a.cap * C::DVp);
   const int64_t meta = sh * (a.cap / 32);
-  // block j straight into LDS buffer j & 1, 1 KB pieces (lane: the 16 bytes that the
+  // block j straight into an LDS buffer, 1 KB pieces (lane: the 16 bytes that the
   // tile's swizzle puts at LDS offset 16 lane)
-  const auto issue = [&](int j) {
-    const uint32_t lds0 = lds_addr(pfa_smem + (j & 1) * C::BUF);
+  const auto issue = [&](int j, int buf) {
+    const uint32_t lds0 = lds_addr(pfa_smem + buf * C::BUF);
     const int64_t k0 = (int64_t)j * PKV_KB;
 #pragma unroll
     for (int u = 0; u < C::NLK; ++u) {
@@ -350,26 +401,48 @@ __global__ __launch_bounds__(64 * NW) void paged_fa_kernel(const PagedAttn a) {
     for (int i = 0; i < 16; ++i) o[v][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;
 
-  if (kb0 < nkb) issue(kb0);
+  // scale factors and missing keys of a block, asked for one block ahead
+  float nkx[2] = {}, nvx[2] = {};
+  uint32_t ngone[2] = {};
+  const auto ask = [&](int j) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int64_t at = meta + 2 * (int64_t)min(j, nkb - 1) + t;
+      nkx[t] = a.kx[at];
+      nvx[t] = a.vx[at];
+      ngone[t] = a.gone[at];
+    }
+  };
+  constexpr int AHEAD = C::NBUF - 1;
+  if (kb0 < nkb) {
+    issue(kb0, 0);
+    if (AHEAD > 1 && kb0 + 1 < nkb) issue(kb0 + 1, 1);
+    ask(kb0);
+  }
+  int buf = 0;
   for (int kb = kb0; kb < nkb; ++kb) {
     // block kb has landed for every wave, and every wave is done with block kb - 1
-    wait_vm<0>();
+    if (AHEAD > 1 && kb + 1 < nkb)
+      wait_vm<C::NLK + C::NLV>();
+    else
+      wait_vm<0>();
     wait_lgkm0();
     lds_barrier();
-    if (kb + 1 < nkb) issue(kb + 1);
+    if (kb + AHEAD < nkb) issue(kb + AHEAD, buf + AHEAD >= C::NBUF ? buf + AHEAD - C::NBUF : buf + AHEAD);
     const int k0 = kb * PKV_KB;
-    if (k0 > s.first + qw + 31) continue;      // behind every query of this wave
-    const char* kt = pfa_smem + (kb & 1) * C::BUF;
+    const char* kt = pfa_smem + buf * C::BUF;
     const char* vt = kt + C::KT;
+    buf = buf + 1 == C::NBUF ? 0 : buf + 1;
     float ct[2], vx[2];
     uint32_t gone[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int64_t at = meta + k0 / 32 + t;
-      ct[t] = fmaxf(cq * a.kx[at], 1.17549435e-38f);   // (a masked score stays -infinity)
-      vx[t] = a.vx[at];
-      gone[t] = a.gone[at];
+      ct[t] = fmaxf(cq * nkx[t], 1.17549435e-38f);   // (a masked score stays -infinity)
+      vx[t] = nvx[t];
+      gone[t] = ngone[t];
     }
+    ask(kb + 1);
+    if (k0 > s.first + qw + 31) continue;      // behind every query of this wave
     // scores: sub-tile t, register i -> key k0 + 32 t + 8 (i / 4) + 4 hi + i % 4
     mla_f32x16 z[2];
 #pragma unroll
@@ -398,13 +471,19 @@ __global__ __launch_bounds__(64 * NW) void paged_fa_kernel(const PagedAttn a) {
       mb = fmaxf(mb, fmaf(mt, ct[t], vx[t]));
     }
     mb = mla_pair_max(mb);
-    const float mn = fmaxf(m, mb);
-    // a query whose keys so far are all masked keeps p = 0 (mn = -inf)
-    const float mc = mn == -INFINITY ? 0.0f : mn;
-    const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mc);
-    const bool moved = m != mn;
-    m = mn;
-    l *= alpha;
+    // the sums stay under an older maximum until some query's grew by 2^8 (p under it)
+    if (__builtin_amdgcn_ballot_w64(mb > m && !(mb - m <= 8.0f))) {
+      const float mn = fmaxf(m, mb);
+      const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[v][i] *= alpha;
+    }
+    // a query whose keys so far are all masked keeps p = 0
+    const float mc = m == -INFINITY ? 0.0f : m;
     f16x8_t pf[4];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -424,13 +503,6 @@ __global__ __launch_bounds__(64 * NW) void paged_fa_kernel(const PagedAttn a) {
         pf[2 * t + half] = __builtin_bit_cast(f16x8_t, w);
       }
       l = fmaf(ls, __builtin_amdgcn_exp2f(-vx[t]), l);
-    }
-    // the accumulators are rescaled only when some lane's maximum moved
-    if (__builtin_amdgcn_ballot_w64(moved)) {
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[v][i] *= alpha;
     }
     // PV: step ps covers keys k0 + 16 ps .. +15 in the order above
     const int gq = lane >> 4, sl = lane & 15;
@@ -561,7 +633,9 @@ size_t paged_kv_carve(PagedAttn& a, const dsmoe_mla_paged_dims* d, Carver& c) {
   a.cap = (int)std::min<int64_t>((int64_t)align_up(std::max(d->max_kv, 1), PKV_ROWS), fit);
   a.slots = (int)std::min<int64_t>(a.p.B, a.p.T / ((int64_t)a.thr + 1));
   if (a.cap == 0 || a.slots == 0) return 0;
-  a.pass = (int)std::min<int64_t>({a.slots, PKV_BYTES / (row * a.cap), 65535});
+  // about 4096 blocks if every slot were full
+  a.kvt = (int)std::min<int64_t>(8, std::max<int64_t>(1, (int64_t)a.slots * a.H * (a.cap / PKV_ROWS) / 2048));
+  a.pass = (int)std::min<int64_t>({a.slots, PKV_BYTES / (row * a.cap), 32767});
   const size_t before = c.off;
   a.slot_of = c.take<int32_t>(a.p.B);
   a.seq_of = c.take<int32_t>(a.slots);
@@ -572,9 +646,9 @@ size_t paged_kv_carve(PagedAttn& a, const dsmoe_mla_paged_dims* d, Carver& c) {
   a.kx = c.take<float>(keys / 32);
   a.vx = c.take<float>(keys / 32);
   a.gone = c.take<uint32_t>(keys / 32);
-  // ranges of keys where the query blocks leave half of the CUs idle
+  // ranges of keys where the query blocks leave half of the places on the CUs idle
   const int64_t items = a.H * cdiv(a.p.T, 32 * pkv_nw(nstep, nv));
-  a.nsp = items >= 128 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({PKV_MAX_SPLITS, 512 / items, a.cap / 128}));
+  a.nsp = (int)std::max<int64_t>(1, std::min<int64_t>({PKV_MAX_SPLITS, (pkv_nw(nstep, nv) == 8 ? 256 : 768) / items, a.cap / 256}));
   if (a.nsp > 1) {
     a.po2 = c.take<float>((size_t)a.nsp * a.p.T * a.H * a.DVp);
     a.ml2 = c.take<float2>((size_t)a.nsp * a.p.T * a.H);
@@ -588,18 +662,27 @@ int launch_paged_plan(const PagedAttn& a, hipStream_t st) {
 }
 
 template <int NS, int NT, bool VEC>
-static void pkv_launch(const PagedAttn& a, bool vpart, hipStream_t st) {
-  auto kern = vpart ? paged_kv_kernel<NS, NT, VEC, true> : paged_kv_kernel<NS, NT, VEC, false>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(a.cap / PKV_ROWS), (unsigned)a.H, (unsigned)a.pass), dim3(256), 0, st, a);
+static int pkv_launch(const PagedAttn& a, int part, hipStream_t st) {
+  constexpr size_t lds = (size_t)NT * 32 * ((NS * 16 + 127) / 128 * 256);
+  static_assert(lds <= 160 * 1024, "LDS");
+  auto kern = paged_kv_kernel<NS, NT, VEC>;
+  if (lds > 64 * 1024) {
+    static const hipError_t attr =
+        hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (attr != hipSuccess) return fail(DSMOE_ERR_HIP, "mla_paged: cannot raise LDS limit");
+  }
+  const unsigned blocks = (unsigned)cdiv(a.cap / PKV_ROWS, a.kvt);
+  hipLaunchKernelGGL(kern, dim3(blocks, (unsigned)a.H, (unsigned)a.pass * (part == 2 ? 2 : 1)), dim3(256), lds, st, a, part);
+  return check_launch("mla_paged_kv");
 }
 
 template <int NS>
-static void pkv_launch_nt(const PagedAttn& a, bool vpart, hipStream_t st) {
-  switch (pkv_nv(vpart ? a.Dv : a.Dn)) {
-    case 1: pkv_launch<NS, 1, true>(a, vpart, st); break;
-    case 2: pkv_launch<NS, 2, true>(a, vpart, st); break;
-    case 4: pkv_launch<NS, 4, true>(a, vpart, st); break;
-    default: pkv_launch<NS, 8, true>(a, vpart, st); break;
+static int pkv_launch_nt(const PagedAttn& a, int part, hipStream_t st) {
+  switch (pkv_nv(part == 1 ? a.Dv : a.Dn)) {
+    case 1: return pkv_launch<NS, 1, true>(a, part, st);
+    case 2: return pkv_launch<NS, 2, true>(a, part, st);
+    case 4: return pkv_launch<NS, 4, true>(a, part, st);
+    default: return pkv_launch<NS, 8, true>(a, part, st);
   }
 }
 
@@ -607,7 +690,7 @@ template <int NSTEP, int NV>
 static int pfa_launch(const PagedAttn& a, hipStream_t st) {
   constexpr int NW = 2 * PfaCfg<NSTEP, NV, 4>::BUF > 80 * 1024 ? 8 : 4;
   using C = PfaCfg<NSTEP, NV, NW>;
-  constexpr size_t lds = 2 * (size_t)C::BUF;
+  constexpr size_t lds = C::NBUF * (size_t)C::BUF;
   static_assert(lds <= 160 * 1024, "LDS");
   auto kern = paged_fa_kernel<NSTEP, NV, NW>;
   if (lds > 64 * 1024) {
@@ -637,22 +720,23 @@ int launch_paged_kv(PagedAttn a, hipStream_t st) {
   const bool vec = a.kvvec && a.wvec;
   for (a.slot0 = 0; a.slot0 < a.slots; a.slot0 += a.pass) {
     a.pass = std::min(a.pass, a.slots - a.slot0);
-    for (bool vpart : {false, true}) {
+    int rc = DSMOE_OK;
+    // in one launch where both parts have as many column tiles
+    const bool one = !vec || pkv_nv(a.Dn) == pkv_nv(a.Dv);
+    for (int part = one ? 2 : 0; part <= 2 && (one || part < 2); ++part) {
       if (!vec) {
-        pkv_launch<16, 8, false>(a, vpart, st);
+        rc = pkv_launch<16, 8, false>(a, part, st);
       } else {
         switch (a.Rq / 16) {
-          case 2: pkv_launch_nt<2>(a, vpart, st); break;
-          case 4: pkv_launch_nt<4>(a, vpart, st); break;
-          case 8: pkv_launch_nt<8>(a, vpart, st); break;
-          case 12: pkv_launch_nt<12>(a, vpart, st); break;
-          default: pkv_launch_nt<16>(a, vpart, st); break;
+          case 2: rc = pkv_launch_nt<2>(a, part, st); break;
+          case 4: rc = pkv_launch_nt<4>(a, part, st); break;
+          case 8: rc = pkv_launch_nt<8>(a, part, st); break;
+          case 12: rc = pkv_launch_nt<12>(a, part, st); break;
+          default: rc = pkv_launch_nt<16>(a, part, st); break;
         }
       }
-      const int rc = check_launch("mla_paged_kv");
       if (rc) return rc;
     }
-    int rc;
     switch (a.DQp / 16) {
       case 2: rc = pfa_launch_nv<2>(a, st); break;
       case 5: rc = pfa_launch_nv<5>(a, st); break;

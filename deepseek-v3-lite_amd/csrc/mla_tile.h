@@ -8,6 +8,7 @@
 namespace dsmoe {
 
 typedef short mla_v4s __attribute__((ext_vector_type(4)));
+typedef float mla_f32x4 __attribute__((ext_vector_type(4)));
 typedef float mla_f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned int mla_u32x4 __attribute__((ext_vector_type(4)));
 
