@@ -25,6 +25,7 @@
 // with a NaN or an infinity has K all NaN and V zero, so that it reaches the queries that
 // see it, through their normaliser, and no other.
 #include <algorithm>
+#include <type_traits>
 
 #include "mla_paged.h"
 #include "mla_tile.h"
@@ -157,21 +158,15 @@ __global__ __launch_bounds__(256) void paged_kv_kernel(const PagedAttn a, int pa
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
       const int i = tid + 256 * u, r = i / (2 * NS), c = i - r * (2 * NS);
-      if (i < NT * 32 * NS * 2) *reinterpret_cast<mla_u32x4*>(pkv_smem + mlb_off(r, c, RB)) = v[u];
+      // (columns past R: zeros against whatever the latent rows' loads repeat)
+      if (i < NT * 32 * NS * 2)
+        *reinterpret_cast<mla_u32x4*>(pkv_smem + mlb_off(r, c, RB)) = 8 * c < a.R ? v[u] : mla_u32x4{0u, 0u, 0u, 0u};
     }
   }
   __syncthreads();
   const MlbLane<RB> lk(lane);
   for (int t = tile0; t < tiles; ++t) {
     const int key = key_of(t);
-    uint32_t nf = 0;
-#pragma unroll
-    for (int st = 0; st < NS; ++st) {
-      if (16 * st + 8 * hi >= a.R) fx[st] = __builtin_bit_cast(bf16x8_t, mla_u32x4{0u, 0u, 0u, 0u});
-      nf = pkv_absmax(__builtin_bit_cast(mla_u32x4, fx[st]), nf);
-    }
-    const uint64_t bl = __builtin_amdgcn_ballot_w64(nf >= 0x7f800000u);
-    const bool bad = (((uint32_t)bl | (uint32_t)(bl >> 32)) >> l32) & 1;
     mla_f32x16 acc[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -181,6 +176,9 @@ __global__ __launch_bounds__(256) void paged_kv_kernel(const PagedAttn a, int pa
       for (int st = 0; st < NS; ++st)
         acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lk.frag(pkv_smem, 32 * j, st), fx[st], acc[j], 0, 0, 0);
     }
+    // a NaN or an infinity in a latent row makes every column one
+    const uint64_t bl = __builtin_amdgcn_ballot_w64(!(fabsf(acc[0][0]) < INFINITY));
+    const bool bad = (((uint32_t)bl | (uint32_t)(bl >> 32)) >> l32) & 1;
     const bool alive = live;
     const uint32_t gone = (uint32_t)__builtin_amdgcn_ballot_w64(gone1);
     const bf16_t* prow = pr;
@@ -220,37 +218,44 @@ __global__ __launch_bounds__(256) void paged_kv_kernel(const PagedAttn a, int pa
         a.gone[meta] = gone;
       }
     }
-    const float nan = __builtin_nanf("");
-    const bool zero = !alive || (vpart && bad);
     // dead rows: zeros (a select: their values may be anything), NaN for K rows that hold one
-    const float f = pkv_pow2(n);
-    const auto put = [&](float v) { return zero ? 0.0f : (!vpart && bad) ? nan : v * f; };
+    const float f = pkv_pow2(n), nan = __builtin_nanf("");
+    const bool zero = !alive || (vpart && bad);
     _Float16* row = vpart ? a.vbuf + (sh * a.cap + key) * a.DVp : a.kbuf + (sh * a.cap + key) * a.DQp;
+    const auto store = [&](auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      const auto put = [&](float v) { return WHOLE ? v * f : zero ? 0.0f : (!vpart && bad) ? nan : v * f; };
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int gp = 0; gp < 2; ++gp) {
-        // columns 32 j + 16 gp + 8 hi .. + 7 of the lane's key: the halves of a register
-        // pair (four columns each of lanes l and l + 32) change places
-        uint32_t u[2][2];
+        for (int gp = 0; gp < 2; ++gp) {
+          // columns 32 j + 16 gp + 8 hi .. + 7 of the lane's key: the halves of a register
+          // pair (four columns each of lanes l and l + 32) change places
+          uint32_t u[2][2];
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+          for (int g = 0; g < 2; ++g)
 #pragma unroll
-          for (int d = 0; d < 2; ++d)
-            u[g][d] = pkv_pack(put(acc[j][8 * gp + 4 * g + 2 * d]), put(acc[j][8 * gp + 4 * g + 2 * d + 1]));
-        const auto r0 = __builtin_amdgcn_permlane32_swap(u[0][0], u[1][0], false, false);
-        const auto r1 = __builtin_amdgcn_permlane32_swap(u[0][1], u[1][1], false, false);
-        const int col = 32 * j + 16 * gp + 8 * hi;
-        const mla_u32x4 o = {(uint32_t)r0[0], (uint32_t)r1[0], (uint32_t)r0[1], (uint32_t)r1[1]};
-        if (col + 8 <= ncols) {
-          *reinterpret_cast<mla_u32x4*>(row + col) = o;
-        } else {
-          const f16x8_t e8 = __builtin_bit_cast(f16x8_t, o);
+            for (int d = 0; d < 2; ++d)
+              u[g][d] = pkv_pack(put(acc[j][8 * gp + 4 * g + 2 * d]), put(acc[j][8 * gp + 4 * g + 2 * d + 1]));
+          const auto r0 = __builtin_amdgcn_permlane32_swap(u[0][0], u[1][0], false, false);
+          const auto r1 = __builtin_amdgcn_permlane32_swap(u[0][1], u[1][1], false, false);
+          const int col = 32 * j + 16 * gp + 8 * hi;
+          const mla_u32x4 o = {(uint32_t)r0[0], (uint32_t)r1[0], (uint32_t)r0[1], (uint32_t)r1[1]};
+          if (WHOLE || col + 8 <= ncols) {
+            *reinterpret_cast<mla_u32x4*>(row + col) = o;
+          } else {
+            const f16x8_t e8 = __builtin_bit_cast(f16x8_t, o);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (col + e < ncols) row[col + e] = e8[e];
+            for (int e = 0; e < 8; ++e)
+              if (col + e < ncols) row[col + e] = e8[e];
+          }
         }
-      }
+    };
+    // the common case without selects and column checks
+    if (ncols == 32 * NT && __builtin_amdgcn_ballot_w64(!alive || bad) == 0)
+      store(std::true_type{});
+    else
+      store(std::false_type{});
     if (vpart) continue;
     for (int d = 8 * hi; d < a.Dr; d += 16) {
       const mla_u32x4 v = pkv_ld8(prow + d, a.Dr - d, VEC);
@@ -560,9 +565,11 @@ __global__ __launch_bounds__(64 * NW) void paged_fa_kernel(const PagedAttn a) {
 }
 
 // The key ranges of a query added by their weights 2^(m_i - max m).  A block: 32 tokens
-// of a block of queries (as numbered for QB = 32) of one head, DVp / 4 lanes a token.
+// of a block of queries (as numbered for QB = 32) of one head, DVp / 4 lanes a token.  N: as
+// many ranges at least.
 constexpr int PKV_MAX_SPLITS = 8;
 
+template <int N>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedAttn a) {
   PagedSeq s;
   int slot, q0;
@@ -570,10 +577,10 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedAttn a) {
   const int h = blockIdx.y, lanes = a.DVp / 4, dv = 4 * ((int)threadIdx.x % lanes);
   for (int q = q0 + (int)threadIdx.x / lanes; q < min(q0 + 32, s.n); q += 256 / lanes) {
     const int64_t grow = (int64_t)(s.t0 + q) * a.H + h, step = (int64_t)a.p.T * a.H;
-    float2 ml[PKV_MAX_SPLITS];
-    float4 v[PKV_MAX_SPLITS];
+    float2 ml[N];
+    float4 v[N];
 #pragma unroll
-    for (int i = 0; i < PKV_MAX_SPLITS; ++i) {
+    for (int i = 0; i < N; ++i) {
       const int64_t p = grow + min(i, a.nsp - 1) * step;
       ml[i] = a.ml2[p];
       v[i] = *reinterpret_cast<const float4*>(a.po2 + p * a.DVp + dv);
@@ -581,9 +588,9 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedAttn a) {
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int i = 0; i < PKV_MAX_SPLITS; ++i) m = fmaxf(m, ml[i].x);
+    for (int i = 0; i < N; ++i) m = fmaxf(m, ml[i].x);
 #pragma unroll
-    for (int i = 0; i < PKV_MAX_SPLITS; ++i) {
+    for (int i = 0; i < N; ++i) {
       if (i >= a.nsp) continue;
       // (a range whose scores are all NaN has no maximum, and a NaN for its sum)
       const float w = ml[i].x != -INFINITY ? __builtin_amdgcn_exp2f(ml[i].x - m) : 0.0f;
@@ -633,8 +640,8 @@ size_t paged_kv_carve(PagedAttn& a, const dsmoe_mla_paged_dims* d, Carver& c) {
   a.cap = (int)std::min<int64_t>((int64_t)align_up(std::max(d->max_kv, 1), PKV_ROWS), fit);
   a.slots = (int)std::min<int64_t>(a.p.B, a.p.T / ((int64_t)a.thr + 1));
   if (a.cap == 0 || a.slots == 0) return 0;
-  // about 4096 blocks if every slot were full
-  a.kvt = (int)std::min<int64_t>(8, std::max<int64_t>(1, (int64_t)a.slots * a.H * (a.cap / PKV_ROWS) / 2048));
+  // about 2048 blocks (K and V) if every slot were full; 1 to 12 tiles a block measure the same
+  a.kvt = (int)std::min<int64_t>(8, std::max<int64_t>(1, (int64_t)a.slots * a.H * (a.cap / PKV_ROWS) / 1024));
   a.pass = (int)std::min<int64_t>({a.slots, PKV_BYTES / (row * a.cap), 32767});
   const size_t before = c.off;
   a.slot_of = c.take<int32_t>(a.p.B);
@@ -702,7 +709,8 @@ static int pfa_launch(const PagedAttn& a, hipStream_t st) {
   hipLaunchKernelGGL(kern, dim3((unsigned)mla_grid(a.H, tiles * a.nsp)), dim3(64 * NW), lds, st, a);
   int rc = check_launch("mla_paged_fa");
   if (rc || a.nsp == 1) return rc;
-  hipLaunchKernelGGL(paged_merge_kernel, dim3((unsigned)(a.p.T / 32 + a.p.B), (unsigned)a.H), dim3(256), 0, st, a);
+  auto merge = a.nsp <= 2 ? paged_merge_kernel<2> : a.nsp <= 4 ? paged_merge_kernel<4> : paged_merge_kernel<PKV_MAX_SPLITS>;
+  hipLaunchKernelGGL(merge, dim3((unsigned)(a.p.T / 32 + a.p.B), (unsigned)a.H), dim3(256), 0, st, a);
   return check_launch("mla_paged_merge");
 }
 
