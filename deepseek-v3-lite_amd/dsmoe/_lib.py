@@ -102,7 +102,8 @@ _SIGNATURES = {
     "dsmoe_mla_attn_bwd_workspace_size": ([ctypes.POINTER(MlaDims)], SZ),
     "dsmoe_mla_attn_kv": ([P, P, P, P, ctypes.POINTER(MlaDims), P, SZ, P], I32),
     "dsmoe_mla_attn_bwd": ([P, P, ctypes.POINTER(MlaDims), P, SZ, P, P, P, P, P, P, P, P, SZ, P], I32),
-    "dsmoe_route_experts": ([P, P, ctypes.POINTER(RouteDims), P, P, P, P], I32),
+    "dsmoe_route_experts_workspace_size": ([ctypes.POINTER(RouteDims)], SZ),
+    "dsmoe_route_experts": ([P, P, ctypes.POINTER(RouteDims), P, P, P, P, SZ, P], I32),
     "dsmoe_route_experts_bwd": ([P, P, P, ctypes.POINTER(RouteDims), P, P], I32),
     "dsmoe_mla_cache_append": ([P, I64, P, I64, I32, P, F32, P, P, P, P, P, ctypes.POINTER(MlaPagedDims), P], I32),
     "dsmoe_mla_attn_paged_workspace_size": ([ctypes.POINTER(MlaPagedDims)], SZ),

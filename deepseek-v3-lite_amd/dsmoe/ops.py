@@ -95,9 +95,12 @@ def _route_fwd(logits, bias, d):
     weights = torch.empty(T, k, dtype=torch.float32, device=dev)
     idx = torch.empty(T, k, dtype=torch.int32, device=dev)
     counts = torch.empty(E, dtype=torch.int32, device=dev)
+    lib = L.load()
+    nbytes = lib.dsmoe_route_experts_workspace_size(d)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with L.on_device(dev):
-        rc = L.load().dsmoe_route_experts(logits.data_ptr(), L.ptr(bias), d, weights.data_ptr(), idx.data_ptr(),
-                                          counts.data_ptr(), L.stream_ptr(dev))
+        rc = lib.dsmoe_route_experts(logits.data_ptr(), L.ptr(bias), d, weights.data_ptr(), idx.data_ptr(),
+                                     counts.data_ptr(), ws.data_ptr(), nbytes, L.stream_ptr(dev))
     if rc:
         L.check(rc, "dsmoe_route_experts")
     return weights, idx, counts

@@ -447,8 +447,9 @@ typedef struct dsmoe_route_dims {
   int32_t normalise;
   float route_scale;
 } dsmoe_route_dims;
+size_t dsmoe_route_experts_workspace_size(const dsmoe_route_dims* dims);   /* needed for counts alone */
 int dsmoe_route_experts(const float* logits, const float* bias, const dsmoe_route_dims* dims, float* weights,
-                        int32_t* idx, int32_t* counts, void* stream);
+                        int32_t* idx, int32_t* counts, void* workspace, size_t workspace_bytes, void* stream);
 int dsmoe_route_experts_bwd(const float* logits, const int32_t* idx, const float* dweights,
                             const dsmoe_route_dims* dims, float* dlogits, void* stream);
 
