@@ -596,15 +596,17 @@ int dsmoe_moe_fwd_kernels(const dsmoe_dims* dims, int training, int32_t* kernels
   return DSMOE_OK;
 }
 
-int dsmoe_moe_fwd(const void* x, const float* gate_w, const float* gate_bias, const void* const* w1,
-                  const void* const* w2, const void* const* w3, const void* const* sw1, const void* const* sw2,
-                  const void* const* sw3, const dsmoe_dims* dims, int training, void* y, int64_t* idx64,
-                  void* weights_x, int32_t* counts, float* logits, void* workspace, size_t workspace_bytes,
-                  void* stream) {
+// The layer with its own gate (ridx null), or on the routing (ridx, rw).
+static int moe_fwd(const void* x, const float* gate_w, const float* gate_bias, const int32_t* ridx, const float* rw,
+                   const void* const* w1, const void* const* w2, const void* const* w3, const void* const* sw1,
+                   const void* const* sw2, const void* const* sw3, const dsmoe_dims* dims, int training, void* y,
+                   int64_t* idx64, void* weights_x, int32_t* counts, float* logits, void* workspace,
+                   size_t workspace_bytes, void* stream) {
   int rc = validate(dims, true);
   if (rc) return rc;
   const dsmoe_dims& d = *dims;
-  DSMOE_REQUIRE(x && gate_w && gate_bias && w1 && w2 && w3 && y, DSMOE_ERR_INVALID, "moe_fwd: NULL required pointer");
+  DSMOE_REQUIRE(x && (ridx ? rw != nullptr : gate_w && gate_bias) && w1 && w2 && w3 && y, DSMOE_ERR_INVALID,
+                "moe_fwd: NULL required pointer");
   DSMOE_REQUIRE(d.S == 0 || (sw1 && sw2 && sw3), DSMOE_ERR_INVALID, "moe_fwd: NULL shared expert pointers");
   const size_t need = dsmoe_moe_fwd_workspace_size(dims, training);
   DSMOE_REQUIRE(workspace && workspace_bytes >= need, DSMOE_ERR_WORKSPACE, "moe_fwd: workspace too small");
@@ -615,7 +617,7 @@ int dsmoe_moe_fwd(const void* x, const float* gate_w, const float* gate_bias, co
   // The weight pointer table goes to the device with the gate launch when it
   // fits one argument chunk and the MFMA gate runs, else with its own launch.
   const int ntab = 3 * d.E + 3 * d.S;
-  const bool tab_in_gate = ntab <= PTR_CHUNK && gate_uses_mfma(x, gate_w, d);
+  const bool tab_in_gate = !ridx && ntab <= PTR_CHUNK && gate_uses_mfma(x, gate_w, d);
   PtrChunk tabc;
   tabc.n = 0;
   tabc.off = 0;
@@ -640,8 +642,11 @@ int dsmoe_moe_fwd(const void* x, const float* gate_w, const float* gate_bias, co
   GateOut go{logits, L.idx, idx64, L.w, weights_x, L.sel, nullptr};
   bool ranked = false;
   tm.begin(ST_GATE);
-  rc = launch_gate(x, nullptr, gate_w, gate_bias, d, go, st, L.gate_part, tab_in_gate ? &tabc : nullptr, L.ptrs, &po,
-                   &ranked);
+  if (ridx)
+    rc = launch_routed_in(ridx, rw, d.T, d.k, d.E, L.idx, L.w, L.sel, st);
+  else
+    rc = launch_gate(x, nullptr, gate_w, gate_bias, d, go, st, L.gate_part, tab_in_gate ? &tabc : nullptr, L.ptrs, &po,
+                     &ranked);
   tm.end();
   if (rc) return rc;
   // (b) permute (counts are the exact per-expert totals, no atomics)
@@ -678,6 +683,24 @@ int dsmoe_moe_fwd(const void* x, const float* gate_w, const float* gate_bias, co
   tm.end();
   tm.call_done(0);
   return rc;
+}
+
+int dsmoe_moe_fwd(const void* x, const float* gate_w, const float* gate_bias, const void* const* w1,
+                  const void* const* w2, const void* const* w3, const void* const* sw1, const void* const* sw2,
+                  const void* const* sw3, const dsmoe_dims* dims, int training, void* y, int64_t* idx64,
+                  void* weights_x, int32_t* counts, float* logits, void* workspace, size_t workspace_bytes,
+                  void* stream) {
+  return moe_fwd(x, gate_w, gate_bias, nullptr, nullptr, w1, w2, w3, sw1, sw2, sw3, dims, training, y, idx64,
+                 weights_x, counts, logits, workspace, workspace_bytes, stream);
+}
+
+int dsmoe_moe_fwd_routed(const void* x, const int32_t* idx, const float* weights, const void* const* w1,
+                         const void* const* w2, const void* const* w3, const void* const* sw1,
+                         const void* const* sw2, const void* const* sw3, const dsmoe_dims* dims, int training, void* y,
+                         void* workspace, size_t workspace_bytes, void* stream) {
+  DSMOE_REQUIRE(idx && weights, DSMOE_ERR_INVALID, "moe_fwd_routed: NULL routing");
+  return moe_fwd(x, nullptr, nullptr, idx, weights, w1, w2, w3, sw1, sw2, sw3, dims, training, y, nullptr, nullptr,
+                 nullptr, nullptr, workspace, workspace_bytes, stream);
 }
 
 // Backward workspace layout (device pointer tables, then buffers).
@@ -793,18 +816,21 @@ int dsmoe_moe_bwd(const void* x, const float* gate_w, const void* const* w1, con
                           dsw1, dsw2, dsw3, dims->dtype, workspace, workspace_bytes, stream);
 }
 
-int dsmoe_moe_bwd_ex(const void* x, const float* gate_w, const void* const* w1, const void* const* w2,
-                     const void* const* w3, const void* const* sw1, const void* const* sw2, const void* const* sw3,
-                     const dsmoe_dims* dims, const void* dy, const void* fwd_workspace, void* dx, float* dgate_w,
-                     void* const* dw1, void* const* dw2, void* const* dw3, void* const* dsw1, void* const* dsw2,
-                     void* const* dsw3, int dw_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+// Of dsmoe_moe_fwd (droute null), or of dsmoe_moe_fwd_routed with the gradient of its weights.
+static int moe_bwd(const void* x, const float* gate_w, const void* const* w1, const void* const* w2,
+                   const void* const* w3, const void* const* sw1, const void* const* sw2, const void* const* sw3,
+                   const dsmoe_dims* dims, const void* dy, const void* fwd_workspace, void* dx, float* dgate_w,
+                   float* droute, void* const* dw1, void* const* dw2, void* const* dw3, void* const* dsw1,
+                   void* const* dsw2, void* const* dsw3, int dw_dtype, void* workspace, size_t workspace_bytes,
+                   void* stream) {
   int rc = validate(dims, true);
   if (rc) return rc;
   const dsmoe_dims& d = *dims;
   DSMOE_REQUIRE(dw_dtype == d.dtype || dw_dtype == DSMOE_F32, DSMOE_ERR_UNSUPPORTED,
                 "moe_bwd: expert weight gradients are written in the compute dtype or fp32");
   const int32_t dw_f32 = dw_dtype == DSMOE_F32 && d.dtype != DSMOE_F32;
-  DSMOE_REQUIRE(x && gate_w && w1 && w2 && w3 && dy && fwd_workspace && dx && dgate_w && dw1 && dw2 && dw3,
+  DSMOE_REQUIRE(x && w1 && w2 && w3 && dy && fwd_workspace && dx && (droute || (gate_w && dgate_w)) && dw1 && dw2 &&
+                    dw3,
                 DSMOE_ERR_INVALID, "moe_bwd: NULL required pointer");
   DSMOE_REQUIRE(d.S == 0 || (sw1 && sw2 && sw3 && dsw1 && dsw2 && dsw3), DSMOE_ERR_INVALID,
                 "moe_bwd: NULL shared expert pointers");
@@ -850,7 +876,9 @@ int dsmoe_moe_bwd_ex(const void* x, const float* gate_w, const void* const* w1, 
     rc = launch_dw_dot(dy, F.o_sorted, F.slot_pos, N, d.k, d.D, d.dtype, B.dw, st);
     if (!rc && B.dy_w) rc = launch_scale_gather_rows(dy, F.sorted_token, F.sorted_w, N, d.D, B.dy_w, st);
   }
-  if (!rc) rc = launch_gate_bwd(B.dw, F.sel, d.T, d.k, d.route_scale, B.dlog, st);
+  if (!rc)
+    rc = droute ? launch_routed_dw(B.dw, F.sel, N, droute, st)
+                : launch_gate_bwd(B.dw, F.sel, d.T, d.k, d.route_scale, B.dlog, st);
   if (!rc) rc = launch_sched32(F.offsets, d.E, BWD_BM, B.sched, B.sched_count, st);
   tm.end();
   if (rc) return rc;
@@ -935,7 +963,7 @@ int dsmoe_moe_bwd_ex(const void* x, const float* gate_w, const void* const* w1, 
     if (rc) return join(rc);
   }
   tm.begin(ST_BWD_GATE);
-  rc = launch_dwgate(x, B.dlog, F.sorted_slot, F.sorted_token, F.offsets, d.E, d.D, d.dtype, dgate_w, ss);
+  if (!droute) rc = launch_dwgate(x, B.dlog, F.sorted_slot, F.sorted_token, F.offsets, d.E, d.D, d.dtype, dgate_w, ss);
   tm.end();
   if (rc) return join(rc);
   // routed dh = w * (dy W2), SwiGLU backward -> [dg | du]
@@ -974,10 +1002,31 @@ int dsmoe_moe_bwd_ex(const void* x, const float* gate_w, const void* const* w1, 
   rc = join(rc);
   if (rc) return rc;
   tm.begin(ST_BWD_REDUCE);
-  rc = launch_dx_final(B.dx_slots, B.dx_shared, B.dlog, F.idx, gate_w, d.T, d.D, d.k, d.dtype, dx, st);
+  rc = launch_dx_final(B.dx_slots, B.dx_shared, droute ? nullptr : B.dlog, F.idx, droute ? nullptr : gate_w,
+                       d.T, d.D, d.k, d.dtype, dx, st);
   tm.end();
   tm.call_done(1);
   return rc;
+}
+
+int dsmoe_moe_bwd_ex(const void* x, const float* gate_w, const void* const* w1, const void* const* w2,
+                     const void* const* w3, const void* const* sw1, const void* const* sw2, const void* const* sw3,
+                     const dsmoe_dims* dims, const void* dy, const void* fwd_workspace, void* dx, float* dgate_w,
+                     void* const* dw1, void* const* dw2, void* const* dw3, void* const* dsw1, void* const* dsw2,
+                     void* const* dsw3, int dw_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  return moe_bwd(x, gate_w, w1, w2, w3, sw1, sw2, sw3, dims, dy, fwd_workspace, dx, dgate_w, nullptr, dw1, dw2, dw3,
+                 dsw1, dsw2, dsw3, dw_dtype, workspace, workspace_bytes, stream);
+}
+
+int dsmoe_moe_bwd_routed(const void* x, const void* const* w1, const void* const* w2, const void* const* w3,
+                         const void* const* sw1, const void* const* sw2, const void* const* sw3,
+                         const dsmoe_dims* dims, const void* dy, const void* fwd_workspace, void* dx, float* dweights,
+                         void* const* dw1, void* const* dw2, void* const* dw3, void* const* dsw1,
+                         void* const* dsw2, void* const* dsw3, int dw_dtype, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+  DSMOE_REQUIRE(dweights, DSMOE_ERR_INVALID, "moe_bwd_routed: NULL dweights");
+  return moe_bwd(x, nullptr, w1, w2, w3, sw1, sw2, sw3, dims, dy, fwd_workspace, dx, nullptr, dweights, dw1, dw2, dw3,
+                 dsw1, dsw2, dsw3, dw_dtype, workspace, workspace_bytes, stream);
 }
 
 // Backward of the operator seam (models/moe_triton.py:438-501).  The forward

@@ -92,7 +92,8 @@ __global__ __launch_bounds__(256) void dx_final_kernel(const T* __restrict__ dx_
   float acc = 0.0f;
   for (int q = 0; q < k; ++q) acc += to_f<T>(dx_slots[(t * k + ord[q]) * (int64_t)D + d]);
   if (dx_shared) acc += to_f<T>(dx_shared[t * (int64_t)D + d]);
-  for (int q = 0; q < k; ++q) acc = fmaf(dlog[t * k + ord[q]], gw[(int64_t)ev[q] * D + d], acc);
+  if (gw)
+    for (int q = 0; q < k; ++q) acc = fmaf(dlog[t * k + ord[q]], gw[(int64_t)ev[q] * D + d], acc);
   dx[t * (int64_t)D + d] = from_f<T>(acc);
 }
 
@@ -137,8 +138,9 @@ struct Vec16<float> {
 // its expert and dlogit); the k slot rows of a column chunk are loaded
 // together before the fp32 sums.
 // KE > 0: k == KE at compile time (k <= 8): every load and sum is
-// unconditional, so the loads stay in flight together.
-template <typename T, int KB, int KE>
+// unconditional, so the loads stay in flight together.  GATE: with the gate's
+// term (else dlog and gw are not read).
+template <typename T, int KB, int KE, bool GATE>
 __global__ __launch_bounds__(256) void dx_final_vec_kernel(const T* __restrict__ dx_slots, const T* __restrict__ dx_shared,
                                                            const float* __restrict__ dlog, const int32_t* __restrict__ idx,
                                                            const float* __restrict__ gw, int D, int k_,
@@ -158,7 +160,7 @@ __global__ __launch_bounds__(256) void dx_final_vec_kernel(const T* __restrict__
     }
     ord_s[q] = j;
     ev_s[q] = e;
-    dl_s[q] = dlog[t * k + j];
+    if (GATE) dl_s[q] = dlog[t * k + j];
   }
   __syncthreads();
   for (int c = threadIdx.x; c * V < D; c += blockDim.x) {
@@ -182,7 +184,7 @@ __global__ __launch_bounds__(256) void dx_final_vec_kernel(const T* __restrict__
       for (int i = 0; i < V; ++i) acc[i] += sv[i];
     }
 #pragma unroll
-    for (int q = 0; q < KB; ++q) {
+    for (int q = 0; GATE && q < KB; ++q) {
       if (q >= k) break;
       const float dl = dl_s[q];
       const float* grow = gw + (int64_t)ev_s[q] * D + d;
@@ -495,7 +497,7 @@ int launch_dx_final(const void* dx_slots, const void* dx_shared, const float* dl
                     int T, int D, int k, int dtype, void* dx, hipStream_t st) {
   if (T == 0) return DSMOE_OK;
   const int V = dtype == DSMOE_BF16 ? 8 : 4;
-  if (D % V == 0 && al16p(dx_slots) && al16p(dx) && al16p(gw) && (!dx_shared || al16p(dx_shared))) {
+  if (D % V == 0 && al16p(dx_slots) && al16p(dx) && (!gw || al16p(gw)) && (!dx_shared || al16p(dx_shared))) {
     const unsigned threads = (unsigned)std::min<int64_t>(256, cdiv(cdiv(D, V), 64) * 64);
     auto go = [&](auto tag) {
       using TT = decltype(tag);
@@ -505,14 +507,14 @@ int launch_dx_final(const void* dx_slots, const void* dx_shared, const float* dl
       switch (k) {
 #define DXF_K(n)                                                                                                   \
   case n:                                                                                                          \
-    hipLaunchKernelGGL((dx_final_vec_kernel<TT, n, n>), dim3((unsigned)T), dim3(threads), 0, st, s, sh, dlog, idx, \
-                       gw, D, k, o);                                                                               \
+    hipLaunchKernelGGL((gw ? dx_final_vec_kernel<TT, n, n, true> : dx_final_vec_kernel<TT, n, n, false>),          \
+                       dim3((unsigned)T), dim3(threads), 0, st, s, sh, dlog, idx, gw, D, k, o);                    \
     break;
         DXF_K(1) DXF_K(2) DXF_K(3) DXF_K(4) DXF_K(5) DXF_K(6) DXF_K(7) DXF_K(8)
 #undef DXF_K
         default:
-          hipLaunchKernelGGL((dx_final_vec_kernel<TT, MAX_TOPK, 0>), dim3((unsigned)T), dim3(threads), 0, st, s, sh,
-                             dlog, idx, gw, D, k, o);
+          hipLaunchKernelGGL((gw ? dx_final_vec_kernel<TT, MAX_TOPK, 0, true> : dx_final_vec_kernel<TT, MAX_TOPK, 0, false>),
+                             dim3((unsigned)T), dim3(threads), 0, st, s, sh, dlog, idx, gw, D, k, o);
       }
     };
     if (dtype == DSMOE_BF16)
@@ -529,6 +531,73 @@ int launch_dx_final(const void* dx_slots, const void* dx_shared, const float* dl
     hipLaunchKernelGGL(dx_final_kernel<float>, dim3(grid), dim3(256), 0, st, static_cast<const float*>(dx_slots),
                        static_cast<const float*>(dx_shared), dlog, idx, gw, T, D, k, static_cast<float*>(dx));
   return check_launch("dx_final");
+}
+
+// A routing that the caller chose, as the layer's kernels need it: k distinct ids in [0, E) per
+// token.  An id outside, or one that the token holds at an earlier slot, gives its place to the
+// lowest id that the token does not hold, with weight 0; used tells which slots stayed.  A thread
+// holds a token's ids in registers.
+__global__ __launch_bounds__(64) void routed_in_kernel(const int32_t* __restrict__ idx, const float* __restrict__ w, int T,
+                                                       int k, int E, int32_t* __restrict__ idx_out,
+                                                       float* __restrict__ w_out, float* __restrict__ used) {
+  const int t = blockIdx.x * 64 + threadIdx.x;
+  if (t >= T) return;
+  const int64_t o = (int64_t)t * k;
+  int e[MAX_TOPK];
+#pragma unroll
+  for (int j = 0; j < MAX_TOPK; ++j) e[j] = j < k ? idx[o + j] : -1;
+  unsigned bad = 0;
+#pragma unroll
+  for (int j = 0; j < MAX_TOPK; ++j) {
+    bool ok = e[j] >= 0 && e[j] < E;
+#pragma unroll
+    for (int i = 0; i < j; ++i) ok = ok && e[i] != e[j];   // an id taken out is -1 by then
+    if (!ok) {
+      e[j] = -1;
+      if (j < k) bad |= 1u << j;
+    }
+  }
+  if (bad) {
+    int next = -1;
+#pragma unroll
+    for (int j = 0; j < MAX_TOPK; ++j) {
+      if (!(bad >> j & 1)) continue;
+      for (bool held = true; held;) {   // ends at an id below E, for k <= E ids are held
+        ++next;
+        held = false;
+#pragma unroll
+        for (int i = 0; i < MAX_TOPK; ++i) held = held || e[i] == next;
+      }
+      e[j] = next;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < MAX_TOPK; ++j) {
+    if (j >= k) break;
+    const bool out = bad >> j & 1;
+    idx_out[o + j] = e[j];
+    w_out[o + j] = out ? 0.0f : w[o + j];
+    used[o + j] = out ? 0.0f : 1.0f;
+  }
+}
+
+__global__ __launch_bounds__(256) void routed_dw_kernel(const float* __restrict__ dw, const float* __restrict__ used,
+                                                        int64_t n, float* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) out[i] = used[i] != 0.0f ? dw[i] : 0.0f;
+}
+
+int launch_routed_in(const int32_t* idx, const float* w, int T, int k, int E, int32_t* idx_out, float* w_out,
+                     float* used, hipStream_t st) {
+  if (T > 0)
+    hipLaunchKernelGGL(routed_in_kernel, dim3((unsigned)cdiv(T, 64)), dim3(64), 0, st, idx, w, T, k, E, idx_out, w_out,
+                       used);
+  return check_launch("routed_in");
+}
+
+int launch_routed_dw(const float* dw, const float* used, int64_t n, float* out, hipStream_t st) {
+  if (n > 0) hipLaunchKernelGGL(routed_dw_kernel, dim3((unsigned)cdiv(n, 256)), dim3(256), 0, st, dw, used, n, out);
+  return check_launch("routed_dw");
 }
 
 // Schedule of height bm from int32 offsets (E + 1) already in device memory.

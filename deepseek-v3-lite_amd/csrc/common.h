@@ -349,8 +349,13 @@ int launch_prep_tok(const void* dy, const void* o_slots, const int32_t* row_of, 
 int launch_gate_bwd(const float* dw, const float* sel, int T, int k, float rs, float* dlog, hipStream_t st);
 int launch_dwgate(const void* x, const float* dlog, const int32_t* sorted_slot, const int32_t* sorted_token,
                   const int32_t* offsets, int E, int D, int dtype, float* dgw, hipStream_t st);
+// dlog and gw null: without the gate's term
 int launch_dx_final(const void* dx_slots, const void* dx_shared, const float* dlog, const int32_t* idx, const float* gw,
                     int T, int D, int k, int dtype, void* dx, hipStream_t st);
+// A given routing into (idx_out, w_out, used), and the gradient of its weights (0 where not used).
+int launch_routed_in(const int32_t* idx, const float* w, int T, int k, int E, int32_t* idx_out, float* w_out,
+                     float* used, hipStream_t st);
+int launch_routed_dw(const float* dw, const float* used, int64_t n, float* out, hipStream_t st);
 int launch_sched32(const int32_t* offsets, int E, int bm, MTile* sched, int32_t* sched_count, hipStream_t st);
 
 }  // namespace dsmoe

@@ -103,7 +103,7 @@ __device__ __forceinline__ uint32_t pkv_pack(float a, float b) {
 // Grid (tiles of 128 positions / a.kvt, H, slots of the pass).  A block keeps its head's weight
 // rows in LDS (mlb_off layout) for a.kvt tiles, whose latent rows are asked for one tile
 // ahead: read by every wave from memory they took 232 us for two prompts of 6144 positions (H 32,
-// R 256, D_nope and D_v 128), this way XXX us.  part: K, V, or 2: by the block's parity.  NT: 32-column tiles,
+// R 256, D_nope and D_v 128), this way 117 us.  part: K, V, or 2: by the block's parity.  NT: 32-column tiles,
 // all computed (LDS rows past the last weight row repeat it and are not stored).  VEC:
 // 16-byte loads of latent, rope and weight rows, every load of a batch issued from a valid
 // address before it is used.

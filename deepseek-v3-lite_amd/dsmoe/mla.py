@@ -421,8 +421,10 @@ def mla_attention_paged(q_nope: torch.Tensor, q_pe: torch.Tensor, kv_pages: torc
     as ``mla_attention`` takes them.  Returns (T, H, D_v) in q_nope's dtype, or writes ``out`` (contiguous bf16).
 
     max_q and max_kv are the most new tokens and the most positions of a sequence, as the scheduler knows them
-    (default: T, and what the table has room for).  They choose kernels and key ranges; no result rests on them.
-    A token that sees no position gives zeros; rows of ``out`` behind the last sequence stay as they were."""
+    (default: T, and what the table has room for).  They choose kernels and size the workspace (K and V of up to max_kv
+    positions, where a sequence has many new tokens); a batch past them is computed all the same.
+    A token that sees no position gives zeros; rows behind the last sequence are not written (of ``out`` they stay as
+    they were)."""
     global hip_calls
     _no_grad("mla_attention_paged", (q_nope, q_pe, kv_pages, pe_pages, wkv_b_k, wkv_b_v, out))
     out_dtype = q_nope.dtype

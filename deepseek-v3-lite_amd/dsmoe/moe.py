@@ -15,7 +15,10 @@ Compute runs only through libdsmoe.so on a ROCm device; a forward on CPU
 tensors raises.  The gate computes fp32 logits from x (bf16 is upcast
 exactly) and the fp32 gate weight.  ``moe_dispatch`` is accepted for config
 compatibility and does not select a backend.  ``shared_inter_dim`` (extension,
-default ``moe_inter_dim``) sets the shared experts' inter width.
+default ``moe_inter_dim``) sets the shared experts' inter width.  ``score_func``
+("sigmoid", "softmax"), ``n_expert_groups`` with ``n_limited_groups`` of them kept,
+``group_score`` and ``norm_topk_prob`` (extensions; the defaults are the reference's
+routing) choose ``ops.route_experts`` in place of the fused gate's routing.
 """
 from __future__ import annotations
 
@@ -90,12 +93,21 @@ class _CachedCast(torch.autograd.Function):
 class AuxLossFreeGate(nn.Module):
     """Sigmoid top-k router with a non-trainable fp32 bias (models/moe.py:7-37)."""
 
+    fused = True   # the reference's routing, in the layer's own kernels
+
     def __init__(self, config: dict):
         super().__init__()
         self.dim = config["dim"]
         self.topk = config["n_activated_experts"]
         self.n_routed_experts = config["n_routed_experts"]
         self.route_scale = config.get("route_scale", 1.0)
+        # extensions (ops.route_experts); with the defaults the fused gate of the reference's routing runs
+        self.score_func = config.get("score_func", "sigmoid")
+        self.n_expert_groups = config.get("n_expert_groups", 1)
+        self.n_limited_groups = config.get("n_limited_groups", self.n_expert_groups)
+        self.group_score = config.get("group_score", "top2")
+        self.norm_topk_prob = config.get("norm_topk_prob", True)
+        self.fused = self.score_func == "sigmoid" and self.n_expert_groups == 1 and bool(self.norm_topk_prob)
         self.bias_upper = config.get("bias_upper_threshold", 0.10)
         self.bias_lower = config.get("bias_lower_threshold", 0.10)
         self.weight = nn.Parameter(torch.empty(self.n_routed_experts, self.dim))
@@ -114,8 +126,18 @@ class AuxLossFreeGate(nn.Module):
         self.bias[counts > avg * (1.0 + self.bias_upper)] -= speed
         self.bias[counts < avg * (1.0 - self.bias_lower)] += speed
 
+    def route(self, x: torch.Tensor):
+        """Weights (T, k) fp32, indices (T, k) int32 and counts (E,) int32 of x (T, dim) under the configured scores and
+        groups, differentiable in x and the weight."""
+        return ops.route_experts(ops.gate_logits(x, _flt(self.weight)), self.topk, _flt(self.bias), score=self.score_func,
+                                 n_groups=self.n_expert_groups, topk_groups=self.n_limited_groups,
+                                 group_score=self.group_score, normalise=self.norm_topk_prob, route_scale=self.route_scale)
+
     def forward(self, x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-        """Normalised top-k weights (x dtype) and int64 expert indices."""
+        """Top-k weights (x dtype) and int64 expert indices."""
+        if not self.fused:
+            w, idx, _ = self.route(x)
+            return w.to(x.dtype), idx.to(torch.int64)
         out = ops.gate_forward(x, _flt(self.weight), _flt(self.bias), self.topk, self.route_scale)
         return out["weights_x"], out["idx64"]
 
@@ -232,15 +254,25 @@ class DeepSeekMoE(nn.Module):
         else:
             weights = [p if p.dtype == cdt else self._cast(p, cdt) for p in params]
         w1, w2, w3, s1, s2, s3 = ops._layer_weights(weights, len(self.experts), len(self.shared_experts))
-        y, idx64, wx, counts = ops.moe_layer(flat.to(cdt), _flt(self.gate.weight), _flt(self.gate.bias), w1, w2, w3,
-                                             s1, s2, s3, k=self.gate.topk, route_scale=self.gate.route_scale,
-                                             master_weights=masters)
+        if self.gate.fused:
+            y, idx64, wx, counts = ops.moe_layer(flat.to(cdt), _flt(self.gate.weight), _flt(self.gate.bias), w1, w2, w3,
+                                                 s1, s2, s3, k=self.gate.topk, route_scale=self.gate.route_scale,
+                                                 master_weights=masters)
+        else:
+            y, idx64, wx, counts = self._routed(flat.to(cdt), (w1, w2, w3, s1, s2, s3), masters)
         self._last_weights = wx.detach().to(flat.dtype)
         self._last_indices = idx64.detach()
         self._last_counts = counts.detach()
         self._counts_of = self._last_indices
         self._stack_dtype = cdt
         return y.to(flat.dtype).view(shape)
+
+    @torch.compiler.disable
+    def _routed(self, x: torch.Tensor, experts, masters):
+        """The layer with the gate's route() in place of the fused gate (not traced by torch.compile)."""
+        w, idx, counts = self.gate.route(x)
+        y = ops.routed_moe_layer(x, w, idx, *experts, master_weights=masters)
+        return y, idx.to(torch.int64), w, counts
 
     # -------------------------------------------------------------- stacked views (read on access)
     def _stack(self, mods, name):

@@ -5,6 +5,7 @@
 * ``gate_forward``, ``route_from_logits``, ``permute``, ``combine``:
   the individual stages, exposed for tests and for callers that compose them.
 * ``route_experts``        routing from logits with softmax scores, groups of experts and its gradient
+* ``gate_logits``, ``routed_moe_layer``  the layer with such a routing between its gate's logits and its experts
 
 Every function requires ROCm device tensors and the built HIP library; there
 is no CPU path.
@@ -465,11 +466,12 @@ def _eager_layer(x, gate_w, gate_bias, weights, masters, E, S, k, route_scale, t
                           bool(masters), x, gate_w, gate_bias, *(masters or weights))
 
 
-def check_layer_args(x: torch.Tensor, gate_w: torch.Tensor, gate_bias: torch.Tensor, w1: Sequence[torch.Tensor],
-                     w2: Sequence[torch.Tensor], w3: Sequence[torch.Tensor], sw1: Sequence[torch.Tensor],
+def check_layer_args(x: torch.Tensor, gate_w: Optional[torch.Tensor], gate_bias: Optional[torch.Tensor],
+                     w1: Sequence[torch.Tensor], w2: Sequence[torch.Tensor], w3: Sequence[torch.Tensor], sw1: Sequence[torch.Tensor],
                      sw2: Sequence[torch.Tensor], sw3: Sequence[torch.Tensor], k: int) -> Tuple[int, int, int, int]:
     """Shapes and dtypes moe_layer's kernels read, checked before any launch:
-    ValueError on a mismatch (the kernels trust these sizes).  -> (E, S, I, I_s)."""
+    ValueError on a mismatch (the kernels trust these sizes); gate_w and gate_bias None
+    for a layer without its own gate.  -> (E, S, I, I_s)."""
     if x.dim() != 2:
         raise ValueError(f"dsmoe: x must be (T, dim), got shape {tuple(x.shape)}")
     if x.dtype not in (torch.float32, torch.bfloat16):
@@ -481,9 +483,9 @@ def check_layer_args(x: torch.Tensor, gate_w: torch.Tensor, gate_bias: torch.Ten
                          f"{len(w1)}, {len(w2)}, {len(w3)}")
     if len(sw2) != S or len(sw3) != S:
         raise ValueError(f"dsmoe: need the same number of shared w1, w2, w3 weights, got {S}, {len(sw2)}, {len(sw3)}")
-    if gate_w.dtype != torch.float32 or tuple(gate_w.shape) != (E, D):
+    if gate_w is not None and (gate_w.dtype != torch.float32 or tuple(gate_w.shape) != (E, D)):
         raise ValueError(f"dsmoe: gate weight must be float32 ({E}, {D}), got {gate_w.dtype} {tuple(gate_w.shape)}")
-    if gate_bias.dtype != torch.float32 or tuple(gate_bias.shape) != (E,):
+    if gate_bias is not None and (gate_bias.dtype != torch.float32 or tuple(gate_bias.shape) != (E,)):
         raise ValueError(f"dsmoe: gate bias must be float32 ({E},), got {gate_bias.dtype} {tuple(gate_bias.shape)}")
     if not 1 <= int(k) <= E:
         raise ValueError(f"dsmoe: need 1 <= n_activated_experts <= {E}, got {k}")
@@ -549,6 +551,133 @@ def moe_layer(x: torch.Tensor, gate_w: torch.Tensor, gate_bias: torch.Tensor, w1
     y, idx64, wx, counts, _ = moe_fwd_op(_c(x), _c(gate_w), _c(gate_bias), ws, masters, E, S, int(k), int(I),
                                          int(I_s), float(route_scale), bool(training))
     return y, idx64, wx, counts
+
+
+# ---------------------------------------------------------------------------- layer on a given routing
+class _GateLogitsFn(torch.autograd.Function):
+    """fp32 logits x W_g^T of the gate's kernels, with their gradient: fp32 products of the dense dlogits, as autocast
+    leaves the reference's gate in fp32 (models/moe.py:32)."""
+
+    @staticmethod
+    def forward(ctx, x, gate_w):
+        ctx.save_for_backward(x, gate_w)
+        return _gate_logits(x, gate_w)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d):
+        x, gate_w = L.restored(ctx.saved_tensors)
+        with torch.autocast(d.device.type, enabled=False):
+            dx = torch.mm(d, gate_w).to(x.dtype) if ctx.needs_input_grad[0] else None
+            dw = torch.mm(d.t().contiguous(), x.float()) if ctx.needs_input_grad[1] else None
+        return dx, dw
+
+
+def _gate_logits(x, gate_w):
+    if x.shape[0] == 0:
+        return torch.empty(0, gate_w.shape[0], dtype=torch.float32, device=x.device)
+    with L.on_device(x.device):
+        zero = torch.zeros(gate_w.shape[0], dtype=torch.float32, device=x.device)
+        return gate_forward(x, gate_w, zero, 1, want_logits=True)["logits"]
+
+
+def gate_logits(x: torch.Tensor, gate_w: torch.Tensor) -> torch.Tensor:
+    """The gate's fp32 logits (T, E) of x (T, D) without its routing, differentiable: for route_experts."""
+    _require_gpu(x, gate_w)
+    if x.dim() != 2 or gate_w.dim() != 2 or gate_w.shape[1] != x.shape[1] or gate_w.dtype != torch.float32:
+        raise ValueError(f"dsmoe: gate_logits needs x (T, D) and a float32 weight (E, D), got {tuple(x.shape)} and "
+                         f"{gate_w.dtype} {tuple(gate_w.shape)}")
+    x, gate_w = _c(x), _c(gate_w)
+    if torch.is_grad_enabled() and (x.requires_grad or gate_w.requires_grad):
+        return _GateLogitsFn.apply(x, gate_w)
+    return _gate_logits(x, gate_w)
+
+
+def _routed_fwd(x, weights, idx, experts, E, S, k, I, I_s, training):
+    dev = x.device
+    y = torch.empty_like(x)
+    if x.shape[0] == 0:
+        return y, torch.empty(0, dtype=torch.uint8, device=dev)
+    d = L.make_dims(x.shape[0], x.shape[1], E, k, I, S, I_s, x.dtype, 1.0)
+    lib = L.load()
+    ws = _ws(lib.dsmoe_moe_fwd_workspace_size(d, int(training)), dev)
+    arrs = [L.ptr_array(a) for a in _layer_weights(experts, E, S)]
+    with L.on_device(dev):
+        rc = lib.dsmoe_moe_fwd_routed(L.ptr(x), L.ptr(idx), L.ptr(weights), *[a[0] for a in arrs], d, int(training), L.ptr(y),
+                                      L.ptr(ws), ws.numel(), L.stream_ptr(dev))
+    L.check(rc, "dsmoe_moe_fwd_routed")
+    return y, ws
+
+
+class _RoutedLayerFn(torch.autograd.Function):
+    """dsmoe_moe_fwd_routed / dsmoe_moe_bwd_routed; leaves are the expert weights, or with masters the masters."""
+
+    @staticmethod
+    def forward(ctx, meta, experts, masters, x, weights, idx, *leaves):
+        y, ws = _routed_fwd(x, weights, idx, experts if masters else leaves, *meta, True)
+        ctx.meta = (*meta, masters)
+        ctx.save_for_backward(x, ws, *(experts if masters else leaves))
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        E, S, k, I, I_s, masters = ctx.meta
+        x, ws, *experts = L.restored(ctx.saved_tensors)
+        dev = x.device
+        T, D = x.shape
+        if T == 0:
+            return (None, None, None, torch.empty_like(x), torch.empty(0, k, dtype=torch.float32, device=dev), None,
+                    *(torch.zeros(w.shape, dtype=torch.float32 if masters else w.dtype, device=dev) for w in experts))
+        d = L.make_dims(T, D, E, k, I, S, I_s, x.dtype, 1.0)
+        lib = L.load()
+        bws = _ws(lib.dsmoe_moe_bwd_workspace_size(d), dev)
+        dy = _c(dy)
+        dx = torch.empty_like(x)
+        dweights = torch.empty(T, k, dtype=torch.float32, device=dev)
+        dws = [torch.empty(w.shape, dtype=torch.float32 if masters else w.dtype, device=dev) for w in experts]
+        arrs = [L.ptr_array(a) for a in (*_layer_weights(experts, E, S), *_layer_weights(dws, E, S))]
+        with L.on_device(dev):
+            rc = lib.dsmoe_moe_bwd_routed(L.ptr(x), *[a[0] for a in arrs[:6]], d, L.ptr(dy), L.ptr(ws), L.ptr(dx),
+                                          L.ptr(dweights), *[a[0] for a in arrs[6:]],
+                                          L.DSMOE_F32 if masters else L.dtype_code(x.dtype), L.ptr(bws), bws.numel(),
+                                          L.stream_ptr(dev))
+        L.check(rc, "dsmoe_moe_bwd_routed")
+        return (None, None, None, dx, dweights, None, *dws)
+
+
+def routed_moe_layer(x: torch.Tensor, weights: torch.Tensor, idx: torch.Tensor, w1: Sequence[torch.Tensor],
+                     w2: Sequence[torch.Tensor], w3: Sequence[torch.Tensor], sw1: Sequence[torch.Tensor] = (),
+                     sw2: Sequence[torch.Tensor] = (), sw3: Sequence[torch.Tensor] = (), *,
+                     master_weights: Optional[Sequence[torch.Tensor]] = None):
+    """moe_layer on a routing that the caller chose (route_experts' weights (T, k) fp32 and idx (T, k)) in place of its
+    gate: the same kernels from the permutation on, gradients to x, the weights and the experts (or their fp32 masters, as
+    moe_layer's).  An id outside [0, E), or one that its token holds at an earlier slot, counts for nothing.
+    Returns y."""
+    E, S, I, I_s = check_layer_args(x, None, None, w1, w2, w3, sw1, sw2, sw3, 1)
+    experts = [*w1, *w2, *w3, *sw1, *sw2, *sw3]
+    dev = _require_gpu(x, weights, idx, *experts)
+    T = x.shape[0]
+    if weights.dim() != 2 or weights.shape[0] != T or weights.shape != idx.shape or idx.is_floating_point():
+        raise ValueError(f"dsmoe: weights and idx must be ({T}, k), idx of integers, got {tuple(weights.shape)} and {idx.dtype} "
+                         f"{tuple(idx.shape)}")
+    k = weights.shape[1]
+    if not 1 <= k <= E:
+        raise ValueError(f"dsmoe: need 1 <= k <= {E}, got {k}")
+    masters = list(master_weights) if master_weights is not None else []
+    if masters and (x.dtype != torch.bfloat16 or len(masters) != len(experts) or any(
+            m.dtype != torch.float32 or m.shape != w.shape for m, w in zip(masters, experts))):
+        raise ValueError("dsmoe: master_weights need bf16 activations and one fp32 master of its shape per expert weight")
+    if any(t.device != dev for t in (weights, idx, *experts, *masters)):
+        raise ValueError("dsmoe: tensors are on different devices")
+    if idx.dtype == torch.int64:
+        idx = idx.clamp(-1, E)   # what lies outside stays outside in 32 bits
+    x, weights, idx = _c(x), _c(weights.float()), _c(idx.to(torch.int32))
+    leaves = masters or [_c(w) for w in experts]
+    experts = [_c(w) for w in experts] if masters else leaves
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, weights, *leaves)):
+        return _RoutedLayerFn.apply((E, S, k, I, I_s), experts if masters else None, bool(masters), x, weights, idx, *leaves)
+    return _routed_fwd(x, weights, idx, experts, E, S, k, I, I_s, False)[0]
 
 
 # ---------------------------------------------------------------------------- operator seam

@@ -203,6 +203,23 @@ int dsmoe_moe_bwd_ex(const void* x, const float* gate_w, const void* const* w1, 
                      void* const* dw1, void* const* dw2, void* const* dw3, void* const* dsw1, void* const* dsw2,
                      void* const* dsw3, int dw_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/* The layer on a routing that the caller chose (dsmoe_route_experts, or any other): idx
+ * (T, k) int32 and weights (T, k) fp32 in place of the gate; route_scale is not read.  An id outside
+ * [0, E), or one that a token holds at an earlier slot, counts for nothing.  Workspaces as
+ * dsmoe_moe_fwd's and dsmoe_moe_bwd's.  The backward writes the gradient of the weights
+ * (dweights (T, k) fp32, 0 for ids that count for nothing) in place of dgate_w, and dx has no part of the
+ * gate's. */
+int dsmoe_moe_fwd_routed(const void* x, const int32_t* idx, const float* weights, const void* const* w1,
+                         const void* const* w2, const void* const* w3, const void* const* sw1,
+                         const void* const* sw2, const void* const* sw3, const dsmoe_dims* dims, int training, void* y,
+                         void* workspace, size_t workspace_bytes, void* stream);
+int dsmoe_moe_bwd_routed(const void* x, const void* const* w1, const void* const* w2, const void* const* w3,
+                         const void* const* sw1, const void* const* sw2, const void* const* sw3,
+                         const dsmoe_dims* dims, const void* dy, const void* fwd_workspace, void* dx, float* dweights,
+                         void* const* dw1, void* const* dw2, void* const* dw3, void* const* dsw1,
+                         void* const* dsw2, void* const* dsw3, int dw_dtype, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 /* f1: aux-loss-free bias update on device (models/moe.py:21-27,194-201).
  * counts (E) int32 -> bias (E) fp32 updated in place by the +/-speed band rule. */
 int dsmoe_update_bias(const int32_t* counts, float* gate_bias, int E, float speed, float upper, float lower,
@@ -389,8 +406,9 @@ typedef struct dsmoe_mla_paged_dims {
   int32_t T, B;
   int32_t H, R, D_nope, D_rope, D_v;   /* H, D_nope, D_v: the attention's alone */
   int32_t pages, page_size, table_width;
-  int32_t max_q;    /* most new tokens of a sequence, and */
-  int32_t max_kv;   /* most positions: they choose kernels and ranges (speed), no result rests on them */
+  int32_t max_q;    /* most new tokens of a sequence: with few of them K and V are never built; and */
+  int32_t max_kv;   /* most positions: the workspace has room to build K and V of that many at once.  Hints alone:
+                     * a batch past them is computed from its latent rows */
   int64_t table_stride;
   int64_t kv_page_stride, kv_row_stride;   /* kv_pages (pages, page_size, R) bf16 */
   int64_t pe_page_stride, pe_row_stride;   /* pe_pages (pages, page_size, D_rope) bf16 */
@@ -411,7 +429,7 @@ int dsmoe_mla_cache_append(const void* ctx_kv, int64_t ctx_kv_stride, const void
 
 /* out (T, H, D_v) bf16: every new token's attention over the positions up to its own
  * (zeros where there is none), dims and weights as dsmoe_mla_attn_fwd_heads (R, D_* <= 256,
- * D_nope + D_rope <= 256); T H < 2^24.  A NaN or an infinity in a cached row reaches the tokens that
+ * D_nope + D_rope <= 256); T H < 2^24, table_width page_size < 2^31 - 2^16.  A NaN or an infinity in a cached row reaches the tokens that
  * see it and no other. */
 size_t dsmoe_mla_attn_paged_workspace_size(const dsmoe_mla_paged_dims* dims);
 int dsmoe_mla_attn_paged(const void* q_nope, const void* q_pe, const void* kv_pages, const void* pe_pages,
