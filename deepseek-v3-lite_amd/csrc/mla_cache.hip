@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256) void mla_cache_append_kernel(const CacheArgs a
   const PagedSeq s = paged_at<PAGED_OFFSETS>(a.p, t, 1, 1, 0);
   const int pos = s.first + t - s.t0;
   // rows behind the last sequence, and positions without a place, are left alone
-  if (s.b < 0 || t - s.t0 >= s.n || pos < 0 || pos >= s.kv) return;
+  if (s.b < 0 || t < s.t0 || t - s.t0 >= s.n || pos < 0 || pos >= s.kv) return;
   int in_page;
   const int page = paged_page(a.p, s.b, pos, in_page);
   if (page < 0) return;
@@ -105,6 +105,7 @@ __global__ __launch_bounds__(256) void mla_cache_append_kernel(const CacheArgs a
 int paged_validate(const dsmoe_mla_paged_dims* d) {
   DSMOE_REQUIRE(d, DSMOE_ERR_INVALID, "mla_paged: NULL dims");
   DSMOE_REQUIRE(d->T >= 0 && d->B >= 0, DSMOE_ERR_INVALID, "mla_paged: T and B must not be negative");
+  DSMOE_REQUIRE(d->B < (1 << 24), DSMOE_ERR_UNSUPPORTED, "mla_paged: 2^24 sequences or more");
   DSMOE_REQUIRE(d->R > 0 && d->D_rope > 0 && d->R <= 256 && d->D_rope <= 256, DSMOE_ERR_INVALID,
                 "mla_paged: R and D_rope must be in 1 .. 256");
   DSMOE_REQUIRE(d->pages > 0 && d->page_size > 0 && d->table_width >= 0, DSMOE_ERR_INVALID,

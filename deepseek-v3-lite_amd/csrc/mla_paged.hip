@@ -88,8 +88,8 @@ __global__ __launch_bounds__(256, 4) void paged_absorb_kernel(const PagedAttn a)
 #pragma unroll
       for (int u = 0; u < U; ++u) v0[u] = pg_ld8(w + (int64_t)min(g + u * groups, a.Dn - 1) * a.R, n, WVEC);
     const PagedSeq s = paged_at<PAGED_ROWS>(a.p, rt, 1, 1, 0);
-    const int i0 = rt - s.r0;
-    if (s.b < 0 || i0 >= s.m) continue;
+    const int i0 = rt - s.r0;   // (below 0: offsets that decrease)
+    if (s.b < 0 || i0 < 0 || i0 >= s.m) continue;
     const int t = s.t0 + i0, row = i0 * a.H + h;
     const bf16_t* qn = a.q_nope + t * a.qn_ts + h * a.qn_hs;
     const bf16_t* qp = a.q_pe + t * a.qp_ts + h * a.qp_hs;
@@ -460,12 +460,13 @@ __global__ __launch_bounds__(256, 4) void paged_out_kernel(const PagedAttn a) {
     const int share = max(a.p.units[a.p.B + 1], 1);
     const PagedSeq s = paged_at<PAGED_ROWS, true>(a.p, rt, 1, 1, 0);
     const int i0 = rt - s.r0;
-    if (s.b < 0 || i0 >= s.m) continue;
+    if (s.b < 0 || i0 < 0 || i0 >= s.m) continue;
     const int row = i0 * a.H + h, mt = row / (16 * a.rt);
     // the units of the row's tile that hold keys it sees, and the blocks that took them
     const int its = (pg_kend(a, s, mt) + a.keys - 1) / a.keys, per = (s.kv + a.keys - 1) / a.keys;
     const int64_t first = s.u0 + (int64_t)mt * per;
-    const int b0 = (int)(first / share), nr = its > 0 ? (int)((first + its - 1) / share) - b0 + 1 : 0;
+    const int b0 = (int)min(first / share, (int64_t)a.blocks - 1);   // (more than 2^31 units: not beyond the buffers)
+    const int nr = its > 0 ? (int)min((first + its - 1) / share, (int64_t)a.blocks - 1) - b0 + 1 : 0;
     const int64_t rows = 16 * a.rt;
     const int64_t p0 = (int64_t)(b0 + pg_tile0(a, s) + mt) * rows + (row - mt * 16 * a.rt);
     bf16_t* orow = a.out + ((int64_t)(s.t0 + i0) * a.H + h) * a.Dv;
@@ -560,8 +561,7 @@ static int pg_validate(const dsmoe_mla_paged_dims* d) {
                 "mla_paged: H must be positive, D_nope and D_v in 1 .. 256");
   DSMOE_REQUIRE(d->D_nope + d->D_rope <= 256, DSMOE_ERR_UNSUPPORTED, "mla_paged: D_nope + D_rope > 256 is not supported");
   DSMOE_REQUIRE(d->H <= 65535, DSMOE_ERR_UNSUPPORTED, "mla_paged: more than 65535 heads");
-  DSMOE_REQUIRE((int64_t)d->T * d->H < (int64_t(1) << 24) && d->B < (1 << 24), DSMOE_ERR_UNSUPPORTED,
-                "mla_paged: T H and B must stay below 2^24");
+  DSMOE_REQUIRE((int64_t)d->T * d->H < (int64_t(1) << 24), DSMOE_ERR_UNSUPPORTED, "mla_paged: T H must stay below 2^24");
   DSMOE_REQUIRE(d->max_kv >= 0 && d->max_q >= 0, DSMOE_ERR_INVALID, "mla_paged: negative max_q or max_kv");
   return DSMOE_OK;
 }

@@ -19,7 +19,8 @@
 // their V rows, the row's own for q.  They return where a scalar costs nothing: kx and
 // q's in the factor of the scores, vx as weight 2^vx in the softmax,
 //   out = sum_j 2^(s_j + vx_j - m) (2^-vx_j v_j) / sum_j 2^(s_j + vx_j - m) 2^-vx_j,
-// m the running maximum of s_j + vx_j, or one up to 2^8 behind it.
+// m the running maximum of s_j + vx_j, or one up to 2^8 behind it.  A row keeps its 11 bits
+// down to 2^-27 of the largest value of its 32 keys.
 //
 // Masked places: a key on no page has its bit in `gone` (and zero rows); a latent row
 // with a NaN or an infinity has K all NaN and V zero, so that it reaches the queries that
@@ -208,7 +209,9 @@ __global__ __launch_bounds__(256) void paged_kv_kernel(const PagedAttn a, int pa
     if (!alive || bad) mx = 0.0f;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
-    const int n = mx > 0.0f ? min(max(13 - ((int)(__float_as_uint(mx) >> 23) - 127), -126), 126) : 0;
+    // (V's at most 2^96: keys' weights are under it in the normaliser, beside those of ordinary
+    // values, and neither the sum of 2^24 of them may pass the range nor one of 2^-24 vanish)
+    const int n = mx > 0.0f ? min(max(13 - ((int)(__float_as_uint(mx) >> 23) - 127), -126), vpart ? 96 : 126) : 0;
     if (lane == 0) {
       const int64_t meta = sh * (a.cap / 32) + t * (PKV_ROWS / 32) + wave;
       if (vpart) {
@@ -302,7 +305,7 @@ __device__ __forceinline__ bool pfa_block(const PagedAttn& a, int tnum, int QB, 
   if (s.b < 0) return false;
   slot = __builtin_amdgcn_readfirstlane(a.slot_of[s.b]) - a.slot0;
   q0 = (tnum - s.t0 / QB - s.b) * QB;
-  return slot >= 0 && slot < a.pass && q0 < s.n;
+  return slot >= 0 && slot < a.pass && q0 >= 0 && q0 < s.n;
 }
 
 template <int NSTEP, int NV, int NW>
@@ -639,7 +642,8 @@ size_t paged_kv_carve(PagedAttn& a, const dsmoe_mla_paged_dims* d, Carver& c) {
   const int64_t fit = PKV_BYTES / row / PKV_ROWS * PKV_ROWS;
   a.cap = (int)std::min<int64_t>((int64_t)align_up(std::max(d->max_kv, 1), PKV_ROWS), fit);
   a.slots = (int)std::min<int64_t>(a.p.B, a.p.T / ((int64_t)a.thr + 1));
-  if (a.cap == 0 || a.slots == 0) return 0;
+  // (grids of attention blocks have room for 2^31 of them)
+  if (a.cap == 0 || a.slots == 0 || (a.p.T / 32 + (int64_t)a.p.B) * (a.H + 7) * PKV_MAX_SPLITS >= (int64_t(1) << 31)) return 0;
   // about 2048 blocks (K and V) if every slot were full; 1 to 12 tiles a block measure the same
   a.kvt = (int)std::min<int64_t>(8, std::max<int64_t>(1, (int64_t)a.slots * a.H * (a.cap / PKV_ROWS) / 1024));
   a.pass = (int)std::min<int64_t>({a.slots, PKV_BYTES / (row * a.cap), 32767});

@@ -423,6 +423,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void route_experts_bwd_kernel(con
 static int route_validate(const dsmoe_route_dims* d) {
   DSMOE_REQUIRE(d, DSMOE_ERR_INVALID, "route_experts: NULL dims");
   DSMOE_REQUIRE(d->T >= 0 && d->E > 0, DSMOE_ERR_INVALID, "route_experts: T must not be negative and E positive");
+  DSMOE_REQUIRE(d->T <= INT32_MAX - 4096, DSMOE_ERR_UNSUPPORTED, "route_experts: too many tokens");
   DSMOE_REQUIRE(d->E <= DSMOE_ROUTE_MAX_EXPERTS, DSMOE_ERR_UNSUPPORTED, "route_experts: more than 512 experts");
   DSMOE_REQUIRE(d->score == DSMOE_SCORE_SIGMOID || d->score == DSMOE_SCORE_SOFTMAX, DSMOE_ERR_INVALID,
                 "route_experts: unknown score");

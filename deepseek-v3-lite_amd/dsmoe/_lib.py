@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import warnings
 from pathlib import Path
 from typing import Iterable, Sequence
@@ -212,6 +213,16 @@ def stream_ptr(device: torch.device):
 
 
 _HERE = contextlib.nullcontext()
+
+
+def eager(fn):
+    """fn called as it is, and as a break of the graph while torch.compile traces (its ctypes calls cannot be traced)."""
+    off = torch.compiler.disable(fn)
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        return off(*args, **kwargs) if torch.compiler.is_compiling() else fn(*args, **kwargs)
+    return call
 
 
 def on_device(device: torch.device):

@@ -372,6 +372,7 @@ def _no_grad(what: str, ts) -> None:
         raise RuntimeError(f"{what} has no backward: call it under torch.no_grad(), or detach its inputs")
 
 
+@L.eager
 def mla_cache_append(ctx_kv: torch.Tensor, ctx_pe: torch.Tensor, kv_pages: torch.Tensor, pe_pages: torch.Tensor,
                      block_table: torch.Tensor, kv_lens: torch.Tensor, q_offsets: torch.Tensor, *,
                      norm_weight: Optional[torch.Tensor] = None, norm_eps: float = 1e-6) -> None:
@@ -411,6 +412,7 @@ def mla_cache_append(ctx_kv: torch.Tensor, ctx_pe: torch.Tensor, kv_pages: torch
         L.check(rc, "dsmoe_mla_cache_append")
 
 
+@L.eager
 def mla_attention_paged(q_nope: torch.Tensor, q_pe: torch.Tensor, kv_pages: torch.Tensor, pe_pages: torch.Tensor,
                         block_table: torch.Tensor, kv_lens: torch.Tensor, q_offsets: torch.Tensor,
                         wkv_b_k: torch.Tensor, wkv_b_v: torch.Tensor, softmax_scale: float, *,

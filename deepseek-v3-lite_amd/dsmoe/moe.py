@@ -267,9 +267,8 @@ class DeepSeekMoE(nn.Module):
         self._stack_dtype = cdt
         return y.to(flat.dtype).view(shape)
 
-    @torch.compiler.disable
     def _routed(self, x: torch.Tensor, experts, masters):
-        """The layer with the gate's route() in place of the fused gate (not traced by torch.compile)."""
+        """The layer with the gate's route() in place of the fused gate."""
         w, idx, counts = self.gate.route(x)
         y = ops.routed_moe_layer(x, w, idx, *experts, master_weights=masters)
         return y, idx.to(torch.int64), w, counts

@@ -137,6 +137,7 @@ class _RouteFn(torch.autograd.Function):
         return dlogits if ctx.dtype == torch.float32 else dlogits.to(ctx.dtype), None, None
 
 
+@L.eager
 def route_experts(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None, *, score: str = "sigmoid",
                   n_groups: int = 1, topk_groups: Optional[int] = None, group_score: str = "top2",
                   normalise: bool = True, route_scale: float = 1.0):
@@ -581,6 +582,7 @@ def _gate_logits(x, gate_w):
         return gate_forward(x, gate_w, zero, 1, want_logits=True)["logits"]
 
 
+@L.eager
 def gate_logits(x: torch.Tensor, gate_w: torch.Tensor) -> torch.Tensor:
     """The gate's fp32 logits (T, E) of x (T, D) without its routing, differentiable: for route_experts."""
     _require_gpu(x, gate_w)
@@ -646,6 +648,7 @@ class _RoutedLayerFn(torch.autograd.Function):
         return (None, None, None, dx, dweights, None, *dws)
 
 
+@L.eager
 def routed_moe_layer(x: torch.Tensor, weights: torch.Tensor, idx: torch.Tensor, w1: Sequence[torch.Tensor],
                      w2: Sequence[torch.Tensor], w3: Sequence[torch.Tensor], sw1: Sequence[torch.Tensor] = (),
                      sw2: Sequence[torch.Tensor] = (), sw3: Sequence[torch.Tensor] = (), *,

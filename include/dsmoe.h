@@ -429,8 +429,10 @@ int dsmoe_mla_cache_append(const void* ctx_kv, int64_t ctx_kv_stride, const void
 
 /* out (T, H, D_v) bf16: every new token's attention over the positions up to its own
  * (zeros where there is none), dims and weights as dsmoe_mla_attn_fwd_heads (R, D_* <= 256,
- * D_nope + D_rope <= 256); T H < 2^24, table_width page_size < 2^31 - 2^16.  A NaN or an infinity in a cached row reaches the tokens that
- * see it and no other. */
+ * D_nope + D_rope <= 256); T H < 2^24, B < 2^24, table_width page_size < 2^31 - 2^16, and of the batch's rows
+ * (token, head), in tiles of 16 or 32, times positions less than 2^41.  A NaN or an infinity in a
+ * cached row reaches the tokens that see it and no other.  Where K and V are built, the values of a key keep 11 bits
+ * down to 2^-27 of the largest of its 32. */
 size_t dsmoe_mla_attn_paged_workspace_size(const dsmoe_mla_paged_dims* dims);
 int dsmoe_mla_attn_paged(const void* q_nope, const void* q_pe, const void* kv_pages, const void* pe_pages,
                          const int32_t* block_table, const int32_t* kv_lens, const int32_t* q_offsets,

@@ -214,6 +214,40 @@ def test_offsets_that_are_out_of_range_stay_inside():
         assert torch.equal(_call(_gpu(x), scale), clean)
 
 
+@pytest.mark.parametrize("H", [4, 31])
+@pytest.mark.parametrize("offsets", [[1, 5, 0, 3], [100, 200, 0, 50], [0, 150, 151, 0], [300, 200, 100, 0], [0, 200, 260, 0]])
+def test_offsets_that_decrease_stay_inside(H, offsets):
+    """Sequences found by a search that offsets in no order mislead: only rows of the batch are written, here and in the pages."""
+    from dsmoe.mla import mla_cache_append
+    x, scale = _batch([60, 200, 1], [300, 260, 64], 16, seed=44, shape=dict(SMALL, H=H), behind=40)
+    g = _gpu(x)
+    g["offsets"] = torch.tensor(offsets, dtype=torch.int32, device=DEV)
+    guard = torch.full((301 + 64, H, 16), 7.0, dtype=torch.bfloat16, device=DEV)
+    for kw in (dict(), dict(max_q=1)):
+        _call(g, scale, out=guard[32:-32], **kw)
+        assert (guard[:32] == 7).all() and (guard[-32:] == 7).all()
+    before = g["kv_pages"].clone()
+    mla_cache_append(torch.randn(301, 16, device=DEV), torch.randn(301, 16, device=DEV), g["kv_pages"], g["pe_pages"], g["table"],
+                     g["kv_lens"], g["offsets"])
+    used = torch.zeros(before.shape[0], dtype=torch.bool)
+    used[x["table"][x["table"] >= 0].long()] = True
+    assert torch.equal(g["kv_pages"].cpu()[~used], before.cpu()[~used])
+
+
+def test_tiny_values_keep_their_weight():
+    """Thousands of keys with values of 1e-36 and 2^-14 of the weight each, beside one with ordinary values: as many together
+    as half of its."""
+    x, scale = _batch([64], [8192], 64, seed=45, shape=MID)
+    pages = x["table"][0].long()
+    x["kv_pages"][pages] = (x["kv_pages"][pages].float() * 1e-36).bfloat16()
+    x["kv_pages"][pages[0], 0] = torch.randn(192, generator=torch.Generator().manual_seed(1)).bfloat16()
+    x["q_nope"].zero_()
+    x["q_pe"].fill_(1.0)
+    x["pe_pages"].zero_()
+    x["pe_pages"][pages[0], 0] = 14 * 0.6931 / (24 * scale)
+    _check(_call(_gpu(x), scale), x, scale)
+
+
 @pytest.mark.parametrize("what", [float("nan"), float("inf"), float("-inf")])
 @pytest.mark.parametrize("n", [9, 150])
 def test_not_finite_rows_reach_those_that_see_them(what, n):
@@ -337,6 +371,19 @@ def test_captured_calls_replay_on_other_lengths_pages_and_values():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(g["kv_pages"], e["kv_pages"])
+
+
+def test_compiled_with_a_graph_break():
+    from dsmoe.mla import mla_cache_append
+    x, scale = _batch([4, 61], [70, 70], 16, seed=46, shape=MID)
+    a, b = _gpu(x), _gpu(x)
+    c, pe = torch.randn(65, 192, device=DEV).bfloat16(), torch.randn(65, 24, device=DEV).bfloat16()
+
+    def f(x, c, pe):
+        mla_cache_append(c, pe, x["kv_pages"], x["pe_pages"], x["table"], x["kv_lens"], x["offsets"])
+        return _call(x, scale) * 2
+    assert torch.equal(torch.compile(f, backend="eager")(a, c, pe), f(b, c, pe))
+    assert torch.equal(a["kv_pages"], b["kv_pages"])
 
 
 def test_two_streams_at_once():

@@ -262,6 +262,29 @@ def test_captured_forward_and_backward():
         assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
+def test_groups_across_lanes_with_as_many_tokens_as_a_block_holds():
+    """64 tokens' keys and group scores in a block's shared memory, more than 64 KiB of it."""
+    x, bias = _inputs(64, 250, seed=17)
+    _check(x, bias, 8, G=10, keep=4)
+
+
+def test_compiled_with_a_graph_break():
+    from dsmoe.ops import route_experts
+    x, bias = _inputs(40, 64, seed=18)
+    b = bias.to(DEV)
+
+    def f(x):
+        w, idx, counts = route_experts(x * 2, 6, b, n_groups=8, topk_groups=3)
+        return w.square().sum(), idx
+    grads = []
+    for fn in (f, torch.compile(f, backend="eager")):
+        leaf = x.to(DEV).requires_grad_(True)
+        y, idx = fn(leaf)
+        y.backward()
+        grads.append((y.detach(), idx, leaf.grad))
+    assert all(torch.equal(p, q) for p, q in zip(*grads))
+
+
 def test_refusals():
     from dsmoe.ops import route_experts
     x, bias = _inputs(4, 64, seed=12)

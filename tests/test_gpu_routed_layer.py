@@ -239,6 +239,18 @@ def test_module_captured():
         assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
+def test_module_compiled():
+    """The operators break the graph; outputs and gradients are the eager module's."""
+    m = _module(GATES[0])
+    f = torch.compile(m, backend="eager")
+    x = torch.randn(20, 64, device=DEV, requires_grad=True)
+    y, z = m(x), f(x)
+    assert torch.equal(y, z)
+    a = torch.autograd.grad(y.square().sum(), [x, *m.parameters()])
+    b = torch.autograd.grad(z.square().sum(), [x, *m.parameters()])
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
 def test_refusals():
     from dsmoe import ops
     x, weights, idx, experts, _ = _inputs(5, 64, 4, 2, 32, 1, torch.bfloat16, seed=7)

@@ -46,6 +46,16 @@ def test_attention_refuses(lib, bad, text):
     assert rc in (L.DSMOE_ERR_INVALID, L.DSMOE_ERR_UNSUPPORTED) and text in lib.dsmoe_last_error()
 
 
+def test_too_many_sequences(lib):
+    import dsmoe._lib as L
+    for call in (lambda d: lib.dsmoe_mla_attn_paged(*[None] * 8, 0, None, 0, d, None, None, 0, None),
+                 lambda d: lib.dsmoe_mla_cache_append(None, 0, None, 0, 1, None, 1e-6, *[None] * 5, d, None)):
+        assert call(_dims(B=1 << 24)) == L.DSMOE_ERR_UNSUPPORTED and b"2^24" in lib.dsmoe_last_error()
+    # K and V are not built where the attention's grid had no room: the workspace is the latent rows' alone
+    few, many = (lib.dsmoe_mla_attn_paged_workspace_size(_dims(T=256, H=16, B=b, max_q=256, max_kv=256)) for b in (1 << 20, (1 << 24) - 1))
+    assert 0 < few and 0 < many
+
+
 def test_pointers_workspace_and_strides_are_checked(lib):
     import dsmoe._lib as L
     d = _dims()

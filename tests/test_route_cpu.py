@@ -30,7 +30,7 @@ def test_struct_matches_the_header():
 
 
 @pytest.mark.parametrize("bad,text", [
-    (dict(T=-1), b"T must"), (dict(E=0), b"E"), (dict(E=513), b"512"), (dict(k=0), b"k must"), (dict(k=17), b"16"),
+    (dict(T=-1), b"T must"), (dict(T=2 ** 31 - 4096), b"too many"), (dict(E=0), b"E"), (dict(E=513), b"512"), (dict(k=0), b"k must"), (dict(k=17), b"16"),
     (dict(E=8, n_groups=1, topk_groups=1, k=9), b"k must"), (dict(n_groups=0), b"n_groups"), (dict(n_groups=7), b"divide"),
     (dict(n_groups=65), b"n_groups"), (dict(topk_groups=0), b"topk_groups"), (dict(topk_groups=9), b"topk_groups"),
     (dict(topk_groups=1, k=9), b"k must"), (dict(score=2), b"score"), (dict(score=-1), b"score")])
@@ -61,7 +61,7 @@ def test_pointers_and_workspace_are_checked(lib):
 
 
 def test_workspace_holds_the_largest_calls_counts(lib):
-    small, large = (lib.dsmoe_route_experts_workspace_size(_dims(T=t, E=512, n_groups=1, topk_groups=1)) for t in (1, 2 ** 31 - 1))
+    small, large = (lib.dsmoe_route_experts_workspace_size(_dims(T=t, E=512, n_groups=1, topk_groups=1)) for t in (1, 2 ** 31 - 4097))
     assert 256 <= small < large < 1 << 34
 
 
