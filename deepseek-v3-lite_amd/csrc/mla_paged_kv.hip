@@ -308,6 +308,13 @@ __device__ __forceinline__ bool pfa_block(const PagedAttn& a, int tnum, int QB, 
   return slot >= 0 && slot < a.pass && q0 >= 0 && q0 < s.n;
 }
 
+// What bounds it: of a SIMD's time on two chunks of 2048 and 1332 tokens behind 4096 and 2641 (H 32, D_nope + D_rope 192, D_v
+// 128; 343 us, 0.89 PFLOP/s of the products that the masks leave), products take 44 % and the softmax's vector
+// instructions as much, and the two waves of a SIMD hardly overlap.  Tried without gain: waves half a
+// block apart (388 us), priorities between the waves of a SIMD, blocks of four waves and 32
+// keys (366), query blocks sorted by their keys (343), 64 queries a wave with the exponentials of
+// one half of the keys beside the products of the other (505: its fragments have no registers to
+// arrive in ahead).
 template <int NSTEP, int NV, int NW>
 __global__ __launch_bounds__(64 * NW) void paged_fa_kernel(const PagedAttn a) {
   using C = PfaCfg<NSTEP, NV, NW>;
@@ -460,6 +467,19 @@ __global__ __launch_bounds__(64 * NW) void paged_fa_kernel(const PagedAttn a) {
 #pragma unroll
       for (int st = 0; st < NSTEP; ++st)
         z[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, lk.frag(kt, 32 * t, st)), qf[st], z[t], 0, 0, 0);
+    }
+    // six fragments on their way (two by the compiler's own order: 357 us for two chunks of 2048
+    // and 1332 tokens behind 4096 and 2641, so 343; the widest values have no registers for them)
+    if constexpr (NV < 8) {
+      constexpr int FRAGS = 2 * NSTEP, EARLY = FRAGS < 6 ? FRAGS : 6;
+      __builtin_amdgcn_sched_group_barrier(0x100, EARLY, 0);   // LDS reads
+#pragma unroll
+      for (int u = 0; u < FRAGS - EARLY; ++u) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);       // a product
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x8, EARLY, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
     if (k0 + PKV_KB > s.kv || k0 + PKV_KB - 1 > s.first + qw || (gone[0] | gone[1])) {
 #pragma unroll

@@ -334,37 +334,34 @@ triton_mla_attention = mla_attention
 # None is read on the host, so a captured call can be replayed on other lengths and pages.
 def _paged_dims(kv_pages, pe_pages, block_table, kv_lens, q_offsets, T: int, new) -> "L.MlaPagedDims":
     """The checked description of a paged batch: ValueError on shapes, types or strides the kernels do not take."""
-    dev = kv_pages.device
+    dev = kv_pages.get_device()
     for t in (kv_pages, pe_pages, block_table, kv_lens, q_offsets, *new):
         if not t.is_cuda:
             raise RuntimeError("mla_paged: tensors must be on a ROCm GPU (no CPU implementation)")
-        if t.device != dev:
+        if t.get_device() != dev:
             raise ValueError("mla_paged: tensors are on different devices")
     if kv_pages.dtype != torch.bfloat16 or pe_pages.dtype != torch.bfloat16:
         raise ValueError(f"mla_paged: pages must be bfloat16 (got {kv_pages.dtype}, {pe_pages.dtype})")
-    if kv_pages.dim() != 3 or pe_pages.dim() != 3 or kv_pages.shape[:2] != pe_pages.shape[:2]:
+    kv_shape, pe_shape, table, lens, offs = kv_pages.shape, pe_pages.shape, block_table.shape, kv_lens.shape, q_offsets.shape
+    if len(kv_shape) != 3 or len(pe_shape) != 3 or kv_shape[:2] != pe_shape[:2]:
         raise ValueError("mla_paged: kv_pages must be (pages, page_size, R) and pe_pages (pages, page_size, D_rope), "
-                         f"got {tuple(kv_pages.shape)} and {tuple(pe_pages.shape)}")
-    if kv_pages.stride(2) != 1 or pe_pages.stride(2) != 1:
+                         f"got {tuple(kv_shape)} and {tuple(pe_shape)}")
+    kv_stride, pe_stride = kv_pages.stride(), pe_pages.stride()
+    if kv_stride[2] != 1 or pe_stride[2] != 1:
         raise ValueError("mla_paged: the rows of the pages must be contiguous")
     for t, name in ((block_table, "block_table"), (kv_lens, "kv_lens"), (q_offsets, "q_offsets")):
         if t.dtype != torch.int32:
             raise ValueError(f"mla_paged: {name} must be int32 (got {t.dtype})")
-    B = kv_lens.size(0) if kv_lens.dim() == 1 else -1
-    if block_table.dim() != 2 or block_table.size(0) != B or q_offsets.dim() != 1 or q_offsets.size(0) != B + 1:
+    B = lens[0] if len(lens) == 1 else -1
+    if len(table) != 2 or table[0] != B or len(offs) != 1 or offs[0] != B + 1:
         raise ValueError("mla_paged: block_table must be (B, W), kv_lens (B,) and q_offsets (B + 1,), got "
-                         f"{tuple(block_table.shape)}, {tuple(kv_lens.shape)} and {tuple(q_offsets.shape)}")
-    if (block_table.stride(1) != 1 and block_table.size(1) > 1) or not kv_lens.is_contiguous() \
-            or not q_offsets.is_contiguous():
+                         f"{tuple(table)}, {tuple(lens)} and {tuple(offs)}")
+    table_stride = block_table.stride()
+    if (table_stride[1] != 1 and table[1] > 1) or not kv_lens.is_contiguous() or not q_offsets.is_contiguous():
         raise ValueError("mla_paged: kv_lens, q_offsets and the rows of block_table must be contiguous")
-    d = L.MlaPagedDims()
-    d.T, d.B = T, B
-    d.pages, d.page_size, d.R = kv_pages.shape
-    d.D_rope, d.table_width = pe_pages.size(2), block_table.size(1)
-    d.table_stride = block_table.stride(0)
-    d.kv_page_stride, d.kv_row_stride = kv_pages.stride(0), kv_pages.stride(1)
-    d.pe_page_stride, d.pe_row_stride = pe_pages.stride(0), pe_pages.stride(1)
-    return d
+    # T, B, H, R, D_nope, D_rope, D_v, pages, page_size, table_width, max_q, max_kv and the strides, in the struct's order
+    return L.MlaPagedDims(T, B, 0, kv_shape[2], 0, pe_shape[2], 0, kv_shape[0], kv_shape[1], table[1], 0, 0, table_stride[0],
+                          kv_stride[0], kv_stride[1], pe_stride[0], pe_stride[1])
 
 
 def _no_grad(what: str, ts) -> None:
@@ -399,15 +396,18 @@ def mla_cache_append(ctx_kv: torch.Tensor, ctx_pe: torch.Tensor, kv_pages: torch
             raise ValueError(f"mla_cache_append: norm_weight must be ({R},) floating, got {tuple(norm_weight.shape)}")
         if norm_weight.dtype != torch.float32 or not norm_weight.is_contiguous():
             norm_weight = norm_weight.float().contiguous()
-    if ctx_kv.stride(1) != 1:
-        ctx_kv = ctx_kv.contiguous()
-    if ctx_pe.stride(1) != 1:
-        ctx_pe = ctx_pe.contiguous()
-    with L.on_device(kv_pages.device):
+    kv_rs, kv_cs = ctx_kv.stride()
+    if kv_cs != 1:
+        ctx_kv, kv_rs = ctx_kv.contiguous(), R
+    pe_rs, pe_cs = ctx_pe.stride()
+    if pe_cs != 1:
+        ctx_pe, pe_rs = ctx_pe.contiguous(), d.D_rope
+    dev = kv_pages.device
+    with L.on_device(dev):
         rc = L.load().dsmoe_mla_cache_append(
-            ctx_kv.data_ptr(), ctx_kv.stride(0), ctx_pe.data_ptr(), ctx_pe.stride(0), L.dtype_code(ctx_kv.dtype),
+            ctx_kv.data_ptr(), kv_rs, ctx_pe.data_ptr(), pe_rs, L.dtype_code(ctx_kv.dtype),
             L.ptr(norm_weight), norm_eps, kv_pages.data_ptr(), pe_pages.data_ptr(), block_table.data_ptr(),
-            kv_lens.data_ptr(), q_offsets.data_ptr(), d, L.stream_ptr(kv_pages.device))
+            kv_lens.data_ptr(), q_offsets.data_ptr(), d, L.stream_ptr(dev))
     if rc:
         L.check(rc, "dsmoe_mla_cache_append")
 
@@ -430,20 +430,23 @@ def mla_attention_paged(q_nope: torch.Tensor, q_pe: torch.Tensor, kv_pages: torc
     global hip_calls
     _no_grad("mla_attention_paged", (q_nope, q_pe, kv_pages, pe_pages, wkv_b_k, wkv_b_v, out))
     out_dtype = q_nope.dtype
-    if q_nope.dim() != 3 or q_pe.dim() != 3 or wkv_b_k.dim() != 3 or wkv_b_v.dim() != 3:
+    shapes = q_nope.shape, q_pe.shape, wkv_b_k.shape, wkv_b_v.shape
+    if any(len(t) != 3 for t in shapes):
         raise ValueError("mla_attention_paged: q_nope, q_pe, wkv_b_k and wkv_b_v must have three dimensions")
-    T, H, D_nope = q_nope.shape
+    T, H, D_nope = shapes[0]
     q_nope, q_pe, wkv_b_k, wkv_b_v = _bf16_inputs((q_nope, q_pe, wkv_b_k, wkv_b_v))
     d = _paged_dims(kv_pages, pe_pages, block_table, kv_lens, q_offsets, T, (q_nope, q_pe, wkv_b_k, wkv_b_v))
-    R, D_rope, D_v = d.R, d.D_rope, wkv_b_v.size(1)
+    R, D_rope, D_v = d.R, d.D_rope, shapes[3][1]
     _check_mla_dim_limits(R, D_nope, D_rope, D_v)
-    if tuple(q_pe.shape) != (T, H, D_rope) or tuple(wkv_b_k.shape) != (H, D_nope, R) or wkv_b_v.size(0) != H \
-            or wkv_b_v.size(2) != R:
+    if shapes[1] != (T, H, D_rope) or shapes[2] != (H, D_nope, R) or shapes[3] != (H, D_v, R):
         raise ValueError("mla_attention_paged: inconsistent shapes")
-    if q_nope.stride(2) != 1:
+    qn, qp = q_nope.stride(), q_pe.stride()
+    if qn[2] != 1:
         q_nope = q_nope.contiguous()
-    if q_pe.stride(2) != 1:
+        qn = q_nope.stride()
+    if qp[2] != 1:
         q_pe = q_pe.contiguous()
+        qp = q_pe.stride()
     if not _head_rows(wkv_b_k):
         wkv_b_k = wkv_b_k.contiguous()
     if not _head_rows(wkv_b_v):
@@ -459,8 +462,8 @@ def mla_attention_paged(q_nope: torch.Tensor, q_pe: torch.Tensor, kv_pages: torc
     d.max_q = T if max_q is None else min(int(max_q), T)
     room = d.table_width * d.page_size
     d.max_kv = min(room if max_kv is None else int(max_kv), room, 0x7fffffff)
-    d.qn_token_stride, d.qn_head_stride = q_nope.stride(0), q_nope.stride(1)
-    d.qp_token_stride, d.qp_head_stride = q_pe.stride(0), q_pe.stride(1)
+    d.qn_token_stride, d.qn_head_stride, _ = qn
+    d.qp_token_stride, d.qp_head_stride, _ = qp
     d.softmax_scale = softmax_scale
     lib = L.load()
     nbytes = lib.dsmoe_mla_attn_paged_workspace_size(d)
