@@ -103,9 +103,12 @@ __device__ __forceinline__ uint32_t pkv_pack(float a, float b) {
 
 // Grid (tiles of 128 positions / a.kvt, H, slots of the pass).  A block keeps its head's weight
 // rows in LDS (mlb_off layout) for a.kvt tiles, whose latent rows are asked for one tile
-// ahead: read by every wave from memory they took 232 us for two prompts of 6144 positions (H 32,
-// R 256, D_nope and D_v 128), this way 117 us.  part: K, V, or 2: by the block's parity.  NT: 32-column tiles,
-// all computed (LDS rows past the last weight row repeat it and are not stored).  VEC:
+// ahead: read by every wave from memory they took 232 us for prompts of 6144 and 3973 positions (H
+// 32, R 256, D_nope and D_v 128, D_rope 64), this way 120 us: 207 MB of K and V written, which
+// alone take 44, and 42 GFLOP.  Without its stores the kernel takes 84, without its products 78: the
+// two blocks of a CU overlap little of either.  Rope rows held in registers so that no load waits
+// behind a store: 122, and 37 against 33 where they cost a block its place on the CU (R 192).
+// part: K, V, or 2: by the block's parity.  NT: 32-column tiles, all computed (LDS rows past the last weight row repeat it and are not stored).  VEC:
 // 16-byte loads of latent, rope and weight rows, every load of a batch issued from a valid
 // address before it is used.
 template <int NS, int NT, bool VEC>
@@ -466,7 +469,8 @@ __global__ __launch_bounds__(64 * NW) void paged_fa_kernel(const PagedAttn a) {
       for (int i = 0; i < 16; ++i) z[t][i] = 0.0f;
 #pragma unroll
       for (int st = 0; st < NSTEP; ++st)
-        z[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, lk.frag(kt, 32 * t, st)), qf[st], z[t], 0, 0, 0);
+        z[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, lk.frag(kt, 32 * t, st)), qf[st], z[t], 0,
+                                                      0, 0);
     }
     // six fragments on their way (two by the compiler's own order: 357 us for two chunks of 2048
     // and 1332 tokens behind 4096 and 2641, so 343; the widest values have no registers for them)
@@ -589,7 +593,7 @@ __global__ __launch_bounds__(64 * NW) void paged_fa_kernel(const PagedAttn a) {
 
 // The key ranges of a query added by their weights 2^(m_i - max m).  A block: 32 tokens
 // of a block of queries (as numbered for QB = 32) of one head, DVp / 4 lanes a token.  N: as
-// many ranges at least.
+// many ranges at least.  7.6 us for 3375 tokens of 12 heads, two ranges of 64 columns (21 MB).
 constexpr int PKV_MAX_SPLITS = 8;
 
 template <int N>
@@ -679,7 +683,8 @@ size_t paged_kv_carve(PagedAttn& a, const dsmoe_mla_paged_dims* d, Carver& c) {
   a.gone = c.take<uint32_t>(keys / 32);
   // ranges of keys where the query blocks leave half of the places on the CUs idle
   const int64_t items = a.H * cdiv(a.p.T, 32 * pkv_nw(nstep, nv));
-  a.nsp = (int)std::max<int64_t>(1, std::min<int64_t>({PKV_MAX_SPLITS, (pkv_nw(nstep, nv) == 8 ? 256 : 768) / items, a.cap / 256}));
+  const int64_t places = pkv_nw(nstep, nv) == 8 ? 256 : 768;
+  a.nsp = (int)std::max<int64_t>(1, std::min<int64_t>({PKV_MAX_SPLITS, places / items, a.cap / 256}));
   if (a.nsp > 1) {
     a.po2 = c.take<float>((size_t)a.nsp * a.p.T * a.H * a.DVp);
     a.ml2 = c.take<float2>((size_t)a.nsp * a.p.T * a.H);
@@ -703,7 +708,8 @@ static int pkv_launch(const PagedAttn& a, int part, hipStream_t st) {
     if (attr != hipSuccess) return fail(DSMOE_ERR_HIP, "mla_paged: cannot raise LDS limit");
   }
   const unsigned blocks = (unsigned)cdiv(a.cap / PKV_ROWS, a.kvt);
-  hipLaunchKernelGGL(kern, dim3(blocks, (unsigned)a.H, (unsigned)a.pass * (part == 2 ? 2 : 1)), dim3(256), lds, st, a, part);
+  const dim3 grid(blocks, (unsigned)a.H, (unsigned)a.pass * (part == 2 ? 2 : 1));
+  hipLaunchKernelGGL(kern, grid, dim3(256), lds, st, a, part);
   return check_launch("mla_paged_kv");
 }
 

@@ -28,6 +28,10 @@ returns each input's gradient in that input's dtype.  fp32 queries outside a
 bf16 autocast region raise ``ValueError`` (the reference layer then uses its
 SDPA path), since rounding them to bf16 would be a precision loss the caller
 did not ask for.
+
+``mla_cache_append`` and ``mla_attention_paged`` serve: the latent rows of many
+sequences in pages, ragged lengths on the device, decoding tokens beside chunks of
+prompts (csrc/mla_cache.hip, csrc/mla_paged.hip, csrc/mla_paged_kv.hip).
 """
 from __future__ import annotations
 
