@@ -373,6 +373,32 @@ def test_captured_calls_replay_on_other_lengths_pages_and_values():
         assert torch.equal(out, want) and torch.equal(g["kv_pages"], e["kv_pages"])
 
 
+def test_captured_as_a_threads_first_call():
+    """Both kinds of sequences in a call that a thread captures before it ever ran one."""
+    import threading
+    x, scale = _batch([2, 70, 1], [40, 170, 9], 16, seed=47, shape=MID)
+    g = _gpu(x)
+    out, want, errors = torch.empty(73, 12, 64, dtype=torch.bfloat16, device=DEV), _call(g, scale), []
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+
+    def run():
+        try:
+            with torch.no_grad(), torch.cuda.graph(graph):
+                _call(g, scale, out=out)
+        except Exception as e:   # noqa: BLE001
+            errors.append(e)
+    t = threading.Thread(target=run)
+    t.start()
+    t.join()
+    assert not errors, errors
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
 def test_compiled_with_a_graph_break():
     from dsmoe.mla import mla_cache_append
     x, scale = _batch([4, 61], [70, 70], 16, seed=46, shape=MID)
