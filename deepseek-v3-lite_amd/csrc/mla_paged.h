@@ -102,6 +102,19 @@ __device__ __forceinline__ int paged_page(const PagedBatch& p, int b, int pos, i
   return page >= 0 && page < p.pages ? page : -1;
 }
 
+// What building K and V saves a sequence of n new tokens and kv positions, up to a factor: the latent rows cost
+// n tokens' way in and out (q W_k, times W_v) and more for every pair, K and V are built for every
+// key, and they meet at n (1 / 72 + 7 / kv) = 1.  Measured with eight sequences of up to n new tokens, H 12,
+// 16, 32 with R 192, 256, 256, us on the latent rows / with K and V: behind 4000 positions n 32 takes
+// 67 / 100, 104 / 180, 199 / 454 and n 128 200 / 110, 353 / 177, 727 / 410 (they meet at 64, 64, 78);
+// behind 500 n 16 takes 30 / 42, 39 / 51, 76 / 90 and n 64 70 / 47, 102 / 57, 209 / 101; fresh
+// prompts of n 32 38 / 32, 53 / 33, 100 / 37.  A batch of both kinds pays for both (behind 500, n up to 32:
+// 45 on the latent rows, 43 with K and V, 66 by each sequence's own gain), so sequences that
+// lie near the line (paged_open) go one way together, by the sum of their gains.
+constexpr int PAGED_FEW = 16;   // K and V are never built for as few tokens
+__host__ __device__ inline int64_t paged_gain(int n, int kv) { return (int64_t)n * ((int64_t)kv + 512) - 72 * (int64_t)kv; }
+__host__ __device__ inline bool paged_open(int n, int kv) { return n > PAGED_FEW && paged_gain(n, kv) > -48 * (int64_t)kv; }
+
 struct PagedAttn {
   PagedBatch p;
   const bf16_t* q_nope;   // row of token t, head h at t qn_ts + h qn_hs
@@ -129,7 +142,6 @@ struct PagedAttn {
   int32_t* units;         // p.units
   int blocks, keys;       // blocks of paged_few_kernel, and keys of a unit
   // on K and V (mla_paged_kv.hip)
-  int thr;                // sequences with more new tokens take them
   int slots, cap;         // sequences at most, and positions of each (a multiple of 128)
   int kvt;                // tiles of 128 positions of a block that builds them
   int slot0, pass;        // the slots of this pass: slot0 .. slot0 + pass - 1

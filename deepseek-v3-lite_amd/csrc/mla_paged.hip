@@ -576,13 +576,11 @@ static int pg_validate(const dsmoe_mla_paged_dims* d) {
 // registers have room for their rope steps.
 static int pg_rt(const PagedAttn& a) { return a.H > 16 && a.Drp <= 64 ? 2 : 1; }
 
-// More new tokens of a sequence than this have its K and V built (mla_paged_kv.hip):
-// for one (head, key) the latent rows cost 6 R + 2 D_rope operations a token (the two
-// parts of q_abs among them) against 2 (D_nope + D_rope + D_v), and K and V 2 R (D_nope + D_v) once.
-static int pg_threshold(const dsmoe_mla_paged_dims* d) {
-  const int64_t build = (int64_t)2 * d->R * (d->D_nope + d->D_v);
-  const int64_t more = 6 * d->R + 2 * d->D_rope - 2 * (d->D_nope + d->D_rope + d->D_v);
-  return more <= 0 ? INT_MAX : (int)std::max<int64_t>(16, build / more);
+// Whether K and V may be built at all: of fewer rows (token, head) the three launches of the latent rows
+// take 24 to 32 us, and those of both kinds 32 to 36, most of it the host's time (a fresh prompt of 32
+// tokens at H 32: 32 / 32, of 96 at H 12: 27 / 33).
+static bool pg_both(const dsmoe_mla_paged_dims* d) {
+  return d->max_q > PAGED_FEW && (int64_t)d->T * d->H >= 1280;
 }
 
 static PagedAttn pg_args(const dsmoe_mla_paged_dims* d, size_t* bytes, void* ws) {
@@ -597,9 +595,8 @@ static PagedAttn pg_args(const dsmoe_mla_paged_dims* d, size_t* bytes, void* ws)
   // not below the smallest normal number: a masked score, -infinity, stays one for a scale of 0
   a.c = std::max((d->softmax_scale < 0.0f ? -d->softmax_scale : d->softmax_scale) * MLA_LOG2E, FLT_MIN);
   Carver c(ws);
-  a.thr = pg_threshold(d);
   const size_t rows = (size_t)a.p.T * a.H;
-  const bool both = d->max_q > a.thr && paged_kv_carve(a, d, c) > 0;
+  const bool both = pg_both(d) && paged_kv_carve(a, d, c) > 0;
   if (!both) a.slots = 0;
   a.rt = pg_rt(a);
   a.keys = 16 * pg_groups(a.Rq / 32) * 4 / a.rt;

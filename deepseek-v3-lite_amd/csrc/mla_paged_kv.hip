@@ -1,9 +1,9 @@
 // The sequences of a paged call (mla_paged.hip) that have many new tokens: K and V of
 // their positions built per head, and the causal flash attention of the chunk on them.
 //
-//   paged_plan_kernel   which sequences those are (more than `thr` new tokens, at most `cap`
-//                       positions, while there are slots), and how the other sequences'
-//                       tokens are numbered.  One wave.
+//   paged_plan_kernel   which sequences those are (paged_open, at most `cap` positions,
+//                       while there are slots), and how the other sequences' tokens are
+//                       numbered.  One wave.
 //   paged_kv_kernel     K = [c W_k^T | pe | 0] and V = c W_v^T of 128 positions of a (slot,
 //                       head), 32 a wave: an MFMA product with the weight rows as first and
 //                       the latent rows as second operand, so a lane holds four consecutive
@@ -44,11 +44,18 @@ __global__ __launch_bounds__(64) void paged_plan_kernel(const PagedAttn a) {
   const int lane = threadIdx.x;
   int slot0 = 0, row0 = 0;
   PagedUnits units;
+  int64_t gain = 0;
+  for (int b = lane; b < a.p.B; b += 64) {
+    const PagedSeq s = paged_seq(a.p, b);
+    if (paged_open(s.n, s.kv)) gain += paged_gain(s.n, s.kv);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) gain += __shfl_xor(gain, d);
   for (int b0 = 0; b0 < a.p.B; b0 += 64) {
     const int b = b0 + lane;
     PagedSeq s = paged_seq(a.p, min(b, a.p.B - 1));
     if (b >= a.p.B) s.n = 0;
-    const bool many = s.n > a.thr && s.kv <= a.cap;
+    const bool many = gain > 0 && paged_open(s.n, s.kv) && s.kv <= a.cap;
     const uint64_t mask = __builtin_amdgcn_ballot_w64(many);
     const int slot = slot0 + __popcll(mask & ((1ull << lane) - 1));
     const bool has = many && slot < a.slots;
@@ -665,7 +672,7 @@ size_t paged_kv_carve(PagedAttn& a, const dsmoe_mla_paged_dims* d, Carver& c) {
   const int64_t row = (int64_t)a.H * (a.DQp + a.DVp) * 2;
   const int64_t fit = PKV_BYTES / row / PKV_ROWS * PKV_ROWS;
   a.cap = (int)std::min<int64_t>((int64_t)align_up(std::max(d->max_kv, 1), PKV_ROWS), fit);
-  a.slots = (int)std::min<int64_t>(a.p.B, a.p.T / ((int64_t)a.thr + 1));
+  a.slots = (int)std::min<int64_t>(a.p.B, a.p.T / (PAGED_FEW + 1));
   // (grids of attention blocks have room for 2^31 of them)
   if (a.cap == 0 || a.slots == 0 || (a.p.T / 32 + (int64_t)a.p.B) * (a.H + 7) * PKV_MAX_SPLITS >= (int64_t(1) << 31)) return 0;
   // about 2048 blocks (K and V) if every slot were full; 1 to 12 tiles a block measure the same

@@ -427,7 +427,7 @@ def mla_attention_paged(q_nope: torch.Tensor, q_pe: torch.Tensor, kv_pages: torc
     as ``mla_attention`` takes them.  Returns (T, H, D_v) in q_nope's dtype, or writes ``out`` (contiguous bf16).
 
     max_q and max_kv are the most new tokens and the most positions of a sequence, as the scheduler knows them
-    (default: T, and what the table has room for).  They choose kernels and size the workspace (K and V of up to max_kv
+    (default: T, or 1 for as many tokens as sequences, and what the table has room for).  They choose kernels and size the workspace (K and V of up to max_kv
     positions, where a sequence has many new tokens); a batch past them is computed all the same.
     A token that sees no position gives zeros; rows behind the last sequence are not written (of ``out`` they stay as
     they were)."""
@@ -463,7 +463,7 @@ def mla_attention_paged(q_nope: torch.Tensor, q_pe: torch.Tensor, kv_pages: torc
             raise ValueError(f"mla_attention_paged: out must be a contiguous bfloat16 ({T}, {H}, {D_v}) on {dev}")
         res = out
     d.H, d.D_nope, d.D_v = H, D_nope, D_v
-    d.max_q = T if max_q is None else min(int(max_q), T)
+    d.max_q = (1 if T == d.B else T) if max_q is None else min(int(max_q), T)
     room = d.table_width * d.page_size
     d.max_kv = min(room if max_kv is None else int(max_kv), room, 0x7fffffff)
     d.qn_token_stride, d.qn_head_stride, _ = qn

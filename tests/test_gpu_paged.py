@@ -106,6 +106,51 @@ def test_chunks(new, kv, page, shape):
     _check(_call(_gpu(x), scale), x, scale)
 
 
+@pytest.mark.parametrize("new,kv,page,shape", [
+    ([300, 130, 17], [300, 131, 300], 37, ODD),          # element loads of queries, latent rows and weights
+    ([400, 300], [400, 461], 16, dict(H=2, R=250, Dn=200, Dr=50, Dv=250)),
+    ([700], [833], 16, dict(H=2, R=128, Dn=16, Dr=240, Dv=256)),
+    ([330, 1, 5], [330, 40, 9], 1, SMALL),
+    ([24, 20, 18, 17, 16, 40], [24, 90, 400, 17, 16, 900], 16, MID),     # near the line, together with K and V
+    ([24, 20, 18, 17, 30, 20], [2000, 90, 900, 1100, 1500, 700], 16, MID),   # and together without
+    ([200, 20, 1], [220, 3000, 700], 64, MID),           # far on either side in one batch
+])
+def test_chunks_of_as_many_rows_as_pay(new, kv, page, shape):
+    """Batches of at least 1280 (token, head) rows, from where on K and V may be built."""
+    assert sum(new) * shape["H"] >= 1280
+    x, scale = _batch(new, kv, page, seed=len(new) + kv[0] + 1, shape=shape)
+    _check(_call(_gpu(x), scale, max_q=max(new), max_kv=max(kv)), x, scale)
+    _check(_call(_gpu(x), scale), x, scale)
+
+
+@pytest.mark.parametrize("scale", [-0.3, 2.0, 0.0])
+def test_scales_of_many_rows(scale):
+    x, _ = _batch([1, 330], [200, 400], 16, seed=48, shape=SMALL)
+    _check(_call(_gpu(x), scale), x, scale)
+
+
+def test_tiny_values_keep_their_weight_in_chunks():
+    """As test_tiny_values_keep_their_weight, with enough rows and tokens for K and V."""
+    x, scale = _batch([128], [8192], 64, seed=49, shape=MID)
+    pages = x["table"][0].long()
+    x["kv_pages"][pages] = (x["kv_pages"][pages].float() * 1e-36).bfloat16()
+    x["kv_pages"][pages[0], 0] = torch.randn(192, generator=torch.Generator().manual_seed(1)).bfloat16()
+    x["q_nope"].zero_()
+    x["q_pe"].fill_(1.0)
+    x["pe_pages"].zero_()
+    x["pe_pages"][pages[0], 0] = 14 * 0.6931 / (24 * scale)
+    _check(_call(_gpu(x), scale), x, scale)
+
+
+def test_offsets_out_of_range_with_many_rows():
+    n = 353
+    x, scale = _batch([2, n], [30, 400], 16, seed=50, shape=SMALL)
+    clean = _call(_gpu(x), scale)
+    for offsets, rows in (([0, 2, 10 ** 9], slice(None)), ([0, 2, -5], slice(0, 2)), ([-9, 2, 2 + n], slice(None))):
+        x["offsets"] = torch.tensor(offsets, dtype=torch.int32)
+        assert (_call(_gpu(x), scale)[rows].float() - clean[rows].float()).abs().max() <= 2e-2 * clean.float().abs().max()
+
+
 def test_chunks_in_several_passes():
     """K and V of one pass hold 4 GiB: a table far wider than the sequences are long."""
     new = [129] * 8 + [1]
@@ -371,6 +416,44 @@ def test_captured_calls_replay_on_other_lengths_pages_and_values():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(g["kv_pages"], e["kv_pages"])
+
+
+def test_captured_chunks_replay_and_streams():
+    """Batches with K and V built: captured and replayed on other lengths, strided inputs with equal bits, two streams at once."""
+    x, scale = _batch([100, 61, 0], [170, 70, 64], 16, seed=51, shape=MID)
+    g = _gpu(x)
+    out = torch.empty(161, 12, 64, dtype=torch.bfloat16, device=DEV)
+    _call(g, scale, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _call(g, scale, out=out)
+    for new, kv in (([100, 61, 0], [170, 70, 64]), ([1, 60, 100], [9, 71, 164]), ([0, 161, 0], [1, 170, 2]), ([40, 60, 61], [40, 80, 61])):
+        g["kv_lens"].copy_(torch.tensor(kv))
+        g["offsets"].copy_(torch.tensor([0, *new]).cumsum(0))
+        g["q_nope"].normal_()
+        want = _call({k: v.clone() for k, v in g.items()}, scale)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    v = dict(g)
+    q = torch.cat([g["q_nope"], g["q_pe"]], -1).transpose(0, 1).contiguous().transpose(0, 1)
+    v["q_nope"], v["q_pe"] = q[..., :48], q[..., 48:]
+    pool = torch.cat([g["kv_pages"], g["pe_pages"]], -1)
+    v["kv_pages"], v["pe_pages"] = pool[..., :192], pool[..., 192:]
+    w = torch.cat([g["w_k"], g["w_v"]], 1)
+    v["w_k"], v["w_v"] = w[:, :48], w[:, 48:]
+    assert torch.equal(_call(v, scale), want)
+    y, _ = _batch([150, 3], [900, 33], 16, seed=52, shape=MID)
+    h, side = _gpu(y), torch.cuda.Stream()
+    other = _call(h, scale)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        with torch.cuda.stream(side):
+            b = _call(h, scale)
+        a = _call(g, scale)
+        torch.cuda.synchronize()
+        assert torch.equal(a, want) and torch.equal(b, other)
 
 
 def test_captured_as_a_threads_first_call():
