@@ -92,9 +92,9 @@ _GROUP_SCORES = {"max": 0, "top2": 1}
 
 
 def _route_fwd(logits, bias, d):
-    T, E, k, dev = d.T, d.E, d.k, logits.device
-    weights = torch.empty(T, k, dtype=torch.float32, device=dev)
-    idx = torch.empty(T, k, dtype=torch.int32, device=dev)
+    shape, E, dev = (d.T, d.k), d.E, logits.device
+    weights = torch.empty(shape, dtype=torch.float32, device=dev)
+    idx = torch.empty(shape, dtype=torch.int32, device=dev)
     counts = torch.empty(E, dtype=torch.int32, device=dev)
     lib = L.load()
     nbytes = lib.dsmoe_route_experts_workspace_size(d)
@@ -164,16 +164,19 @@ def route_experts(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = N
         raise ValueError(f"route_experts: score must be one of {tuple(_SCORES)} and group_score of {tuple(_GROUP_SCORES)}, "
                          f"got {score!r} and {group_score!r}")
     if bias is not None:
-        if tuple(bias.shape) != (E,):
+        if bias.shape != (E,):
             raise ValueError(f"route_experts: bias must be ({E},), got {tuple(bias.shape)}")
-        bias = bias.detach()
+        if bias.requires_grad:
+            bias = bias.detach()
         if bias.dtype != torch.float32 or not bias.is_contiguous():
             bias = bias.float().contiguous()
     d = L.RouteDims(T, E, int(k), _SCORES[score], int(n_groups), int(n_groups if topk_groups is None else topk_groups),
                     _GROUP_SCORES[group_score], 1 if normalise else 0, float(route_scale))
     if torch.is_grad_enabled() and logits.requires_grad:
         return _RouteFn.apply(logits, bias, d)
-    return _route_fwd(_c(logits.detach().float()), bias, d)
+    if logits.requires_grad:
+        logits = logits.detach()
+    return _route_fwd(_c(logits if logits.dtype == torch.float32 else logits.float()), bias, d)
 
 
 def check_routing(idx: torch.Tensor, E: int) -> None:
